@@ -8,12 +8,15 @@ of that name beside this directory loads it; the directory name itself is not an
 from .backend import BackendSettings, make_backend_class
 from .capability import (
     CapabilityError,
+    DECODE_CAPABILITY,
     GENERALIZATION_CAPABILITY,
     KV_HEAD_SHARD_CAPABILITY,
     OperatorCapability,
     V1_CAPABILITY,
     check_supported,
 )
+from .decode import DecodeWorkspace, check_decode, paged_decode, plan_decode_workspace
+from .eviction import WeightsWorkspace, evict_lightest, extend_weights, plan_weights_workspace
 from .kernel import NativeError, build, load, source_build_id
 from .ops import (PrefillRequest, check_request, plan_batch_workspace, plan_workspace, prefill_extend,
                   prefill_extend_batch)
@@ -27,6 +30,8 @@ __all__ = [
     "check_request", "plan_workspace", "plan_batch_workspace", "prefill_extend", "prefill_extend_batch",
     "CapacityPlan", "BatchPlan", "FP8PrefillBatchWorkspace",
     "FP8PrefillWorkspace", "WorkspaceCapacityError", "BackendSettings", "make_backend_class", "fp8_paged_prefill",
+    "DECODE_CAPABILITY", "DecodeWorkspace", "check_decode", "paged_decode", "plan_decode_workspace",
+    "WeightsWorkspace", "evict_lightest", "extend_weights", "plan_weights_workspace",
 ]
 
 __version__ = "0.1.0"

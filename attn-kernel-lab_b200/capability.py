@@ -121,6 +121,28 @@ KV_HEAD_SHARD_CAPABILITY = OperatorCapability(
 )
 
 
+#: Heads of the decode side (`paged_decode`) and of the attention weights of an extend
+#: (`extend_weights`): up to eight query heads share a kv head, which covers the declared family, its
+#: kv-head shards and the tested ratios.  No counterpart in the reference.
+_GROUPS, _DECODE_KV = range(1, 9), (1, 2, 4, 8)
+DECODE_CAPABILITY = OperatorCapability(
+    operator_contract_version=1,
+    layout_version=LAYOUT_VERSION,
+    head_dim=(256,),
+    q_heads=tuple(sorted({kv * g for kv in _DECODE_KV for g in _GROUPS})),
+    kv_heads=_DECODE_KV,
+    page_size=(1,),
+    modes=("decode", "extend_weights"),
+    masks=("bottom_right_causal",),
+    returns_lse=True,
+    kv_dtypes=("bfloat16", "float16"),
+    cuda_graph=CUDA_GRAPH_DECLARED,
+    notes=("The pool is read in its own type; nothing is quantised.",
+           "CUDA graph capture needs a planned workspace and caller-owned outputs; lengths, rows and "
+           "page-table entries are read on the device at replay."),
+)
+
+
 def check_supported(
     *,
     head_dim: int,

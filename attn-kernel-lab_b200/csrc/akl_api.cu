@@ -213,6 +213,11 @@ BatchRef make_ref(const akl_batch_t* b, const BatchLayout& L, void* table) {
   return r;
 }
 
+int need_q(const akl_call_t* c) { return (c->q == nullptr) ? AKL_ERR_INVALID : AKL_OK; }
+int need_out(const akl_call_t* c) { return (c->out == nullptr) ? AKL_ERR_INVALID : AKL_OK; }
+
+}  // namespace
+
 int device_sm_count(int* out) {
   static std::atomic<int> cached[64];
   int dev = 0;
@@ -227,11 +232,6 @@ int device_sm_count(int* out) {
   *out = n;
   return AKL_OK;
 }
-
-int need_q(const akl_call_t* c) { return (c->q == nullptr) ? AKL_ERR_INVALID : AKL_OK; }
-int need_out(const akl_call_t* c) { return (c->out == nullptr) ? AKL_ERR_INVALID : AKL_OK; }
-
-}  // namespace
 
 // Every host-side check of the whole-operator entry, with no CUDA call: shared by
 // akl_prefill_extend and the entry that works out of the library's own scratch.

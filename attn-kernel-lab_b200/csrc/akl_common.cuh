@@ -345,6 +345,13 @@ __device__ __forceinline__ long long load_idx(const void* idx, int i) {
   return static_cast<long long>(reinterpret_cast<const int*>(idx)[i]);
 }
 
+// Entry i of an index array whose type is only known at run time (uniform over the launch).
+__device__ __forceinline__ long long load_index(const void* idx, int dtype, long long i) {
+  return dtype == AKL_IDX_I64 ? __ldg(reinterpret_cast<const long long*>(idx) + i)
+                              : static_cast<long long>(__ldg(reinterpret_cast<const int*>(idx) + i));
+}
+inline bool known_index(int dtype) { return dtype == AKL_IDX_I64 || dtype == AKL_IDX_I32; }
+
 // host-side launchers (one translation unit each)
 int launch_kv_tile_stats(const Geom& g, int kv_dtype, int idx_dtype, cudaStream_t s, bool with_q = false);
 int launch_kv_means(const Geom& g, cudaStream_t s, bool fuse_scales = false);
@@ -359,6 +366,7 @@ int launch_batch_means(const BatchRef& b, int kv_heads, cudaStream_t s);
 int launch_batch_transform(const BatchRef& b, int kv_dtype, int idx_dtype, int sm_count, cudaStream_t s);
 int launch_batch_attention(const BatchRef& b, bool qk_i8, int sm_count, cudaStream_t s);
 int launch_exact_division_selftest(const float* scales, int n, unsigned long long* mismatches, cudaStream_t s);
+int device_sm_count(int* out);
 void note_cuda_error(cudaError_t e, const char* where);
 int validate_prefill_call(const akl_call_t* c, Geom* g);
 

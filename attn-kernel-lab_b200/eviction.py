@@ -1,0 +1,258 @@
+"""Bounding a request's cache by what its tokens were attended to.
+
+`extend_weights` adds up what the query rows of an extend (all of them, or the last ones as a window)
+put on every cached position, from the log-sum-exp that `prefill_extend` returns; `paged_decode` with
+`weights` goes on with the same accumulator token by token.  `evict_lightest` then shortens page-table
+rows to the heaviest positions, in place, and lists the slots that became free.  The pool itself is
+never moved: a slot is a page.
+
+The reference has no counterpart; validation, errors, workspaces and streams are those of `ops`.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .capability import DECODE_CAPABILITY, OperatorCapability
+from .decode import (_INDEX, _KV, _Scratch, _call, _check_batch_vector, _check_decay, _check_heads, _check_rows,
+                     _check_scale, _check_sizes, _check_table, _need, _need_cuda, _pool_stride, _raise_on_status,
+                     _row_stride)
+from .ops import _dtype_name, _reject, _same_device, _shares_storage
+
+__all__ = ["WeightsWorkspace", "evict_lightest", "extend_weights", "plan_weights_workspace"]
+
+
+class WeightsWorkspace(_Scratch):
+    """Capacity-reserved scratch of `extend_weights`; one call at a time (stream order) may use it."""
+
+    def __init__(self, device, *, max_kv_len: int, max_q_len: int, q_heads: int, kv_heads: int):
+        from . import kernel
+
+        _check_sizes(max_kv_len=max_kv_len, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
+        self.plan = kernel.WeightsPlan(max_kv_len, max_q_len, q_heads, kv_heads)
+        layout = kernel.WeightsLayout()
+        kernel.check(kernel.load().akl_weights_layout(ctypes.byref(self.plan), ctypes.byref(layout)),
+                     "akl_weights_layout")
+        super().__init__(device, layout)
+
+
+def plan_weights_workspace(device, *, max_kv_len: int, max_q_len: int, q_heads: int | None = None,
+                           kv_heads: int | None = None, capability: OperatorCapability = DECODE_CAPABILITY):
+    """A `WeightsWorkspace` for extends within the two maxima; heads default to 32:4 and are validated
+    against the declared surface."""
+    q_heads = 32 if q_heads is None else int(q_heads)
+    kv_heads = 4 if kv_heads is None else int(kv_heads)
+    _check_heads(q_heads, kv_heads, max(capability.head_dim), capability.kv_dtypes[0], "extend_weights", False,
+                 capability)
+    return WeightsWorkspace(device, max_kv_len=max_kv_len, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
+
+
+def _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale, capability) -> None:
+    device = q.device if isinstance(q, torch.Tensor) else None
+    _need("q", q, (torch.bfloat16,), 3, device, "[q_len, q_heads, head_dim]")
+    if not isinstance(k_pool, torch.Tensor) or k_pool.dim() != 3:
+        _need("k_pool", k_pool, _KV, 3, device, "[pool, kv_heads, head_dim]")
+    q_len, q_heads, head_dim = q.shape
+    kv_heads = k_pool.shape[1]
+    _check_heads(q_heads, kv_heads, head_dim, _dtype_name(k_pool.dtype), "extend_weights", False, capability)
+    _need("k_pool", k_pool, _KV, 3, device, "[pool, kv_heads, head_dim]")
+    if k_pool.shape[2] != head_dim:
+        _reject(f"k_pool head_dim {k_pool.shape[2]} must equal q head_dim {head_dim}", field="k_pool",
+                value=int(k_pool.shape[2]), supported=head_dim)
+    if q_len < 1 or k_pool.shape[0] < 1:
+        _reject(f"q_len must be >= 1 and the pool must hold a slot, got {q_len} and {k_pool.shape[0]}", field="q_len",
+                value=q_len, supported=">= 1")
+    _check_rows("q", q, q_heads)
+    _check_rows("k_pool", k_pool, kv_heads)
+    _need("idx", idx, _INDEX, 1, device, "[kv_len]")
+    kv_len = idx.shape[0]
+    if kv_len < 1 or not idx.is_contiguous():
+        _reject(f"idx must be contiguous and name at least one position, got {kv_len} with stride {idx.stride()}",
+                field="idx", value=kv_len, supported=">= 1, contiguous")
+    if isinstance(prefix, bool) or not isinstance(prefix, int):
+        _reject(f"prefix must be a Python int, got {type(prefix).__name__}", field="prefix",
+                value=type(prefix).__name__, supported="int")
+    if not 0 <= prefix <= kv_len - q_len:
+        _reject(f"prefix={prefix} is outside [0, kv_len - q_len] = [0, {kv_len - q_len}] for kv_len={kv_len}, "
+                f"q_len={q_len}", field="prefix", value=prefix, supported=(0, kv_len - q_len))
+    _need("lse", lse, (torch.float32,), 2, device, "[q_len, q_heads]")
+    if lse.shape != q.shape[:2] or not lse.is_contiguous():
+        _reject(f"lse must be contiguous {(q_len, q_heads)}, got {tuple(lse.shape)} with strides "
+                f"{tuple(lse.stride())}", field="lse", value=tuple(lse.shape), supported=(q_len, q_heads))
+    _need("weights", weights, (torch.float32,), 1, device, "[kv_len]")
+    if weights.shape[0] != kv_len or not weights.is_contiguous():
+        _reject(f"weights must be contiguous [{kv_len}], got {tuple(weights.shape)} with stride {weights.stride()}",
+                field="weights", value=tuple(weights.shape), supported=(kv_len,))
+    if _shares_storage(weights, lse):
+        _reject("weights must not overlap lse storage", field="weights", value="aliases lse",
+                supported="a distinct allocation")
+    _check_decay(weight_decay)
+    if sm_scale is not None:
+        _check_scale(sm_scale)
+    if workspace is not None:
+        if not isinstance(workspace, WeightsWorkspace):
+            _reject(f"workspace must be a WeightsWorkspace or None, got {type(workspace).__name__}",
+                    field="workspace", value=type(workspace).__name__, supported="WeightsWorkspace | None")
+        if not _same_device(workspace.device, device):
+            _reject(f"workspace is on {workspace.device} but q is on {device}", field="workspace",
+                    value=str(workspace.device), supported=str(device))
+
+
+def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float = 1.0, workspace=None, sm_scale=None,
+                   capability: OperatorCapability = DECODE_CAPABILITY, check_status: bool = False):
+    """Attention weight of every cached position under the query rows of an extend, in place.
+
+    `q` [q_len, q_heads, 256] BF16, `k_pool` [pool, kv_heads, 256] BF16 or FP16, `idx` [kv_len] int32 or
+    int64 and `prefix` as in `prefill_extend`: row t sees the positions 0 .. prefix + t.  `lse` [q_len,
+    q_heads] FP32 base 2 is what that call returned (of any softmax over the same scores).  `weights`
+    [kv_len] FP32 becomes `weight_decay` times itself plus
+
+        sum over t, h with i <= prefix + t of 2^(sm_scale log2e <q[t, h], k_i> - lse[t, h]).
+
+    A row whose `lse` is infinite adds nothing (it saw no key); a slot outside the pool gets no weight.
+    To judge by a window of w rows pass `q[-w:]`, `lse[-w:]` and `prefix + q_len - w`.  The sum has a
+    fixed order: equal inputs give equal bits.
+
+    Enqueues on the current stream and does not synchronise unless `check_status` (a debugging aid).
+    Returns `weights`."""
+    _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale, capability)
+    device = q.device
+    _need_cuda("extend_weights", device)
+    from . import kernel
+
+    lib = kernel.load()
+    q_len, q_heads = q.shape[:2]
+    kv_heads, kv_len = k_pool.shape[1], idx.shape[0]
+    if workspace is None:
+        workspace = WeightsWorkspace(device, max_kv_len=kv_len, max_q_len=q_len, q_heads=q_heads, kv_heads=kv_heads)
+    else:
+        p = workspace.plan
+        if kv_len > p.max_kv_len or q_len > p.max_q_len or (q_heads, kv_heads) != (p.q_heads, p.kv_heads):
+            from .quant import WorkspaceCapacityError
+
+            raise WorkspaceCapacityError(
+                f"extend of {q_len} rows over {kv_len} positions at {q_heads}:{kv_heads} heads is outside the "
+                f"workspace plan (max_q_len={p.max_q_len}, max_kv_len={p.max_kv_len}, heads "
+                f"{p.q_heads}:{p.kv_heads}); the allocation never changes")
+    call = kernel.Weights(
+        q.data_ptr(), k_pool.data_ptr(), idx.data_ptr(), lse.data_ptr(), weights.data_ptr(), workspace._ptr,
+        workspace._bytes, workspace.plan, k_pool.shape[0], q.stride(0) if q_len > 1 else q_heads * 256,
+        _pool_stride(k_pool), q_len, kv_len, prefix, q_heads, kv_heads, _KV[k_pool.dtype], _INDEX[idx.dtype],
+        1.0 / 16.0 if sm_scale is None else sm_scale, weight_decay)
+    _call(device, lib.akl_extend_weights, "akl_extend_weights", call)
+    if check_status:
+        _raise_on_status(workspace, "akl_extend_weights")
+    return weights
+
+
+def _check_out(name, t, like, source_name) -> None:
+    """An output table: the input itself, or a tensor of its shape that shares nothing with it."""
+    if t is like:
+        return
+    _need(name, t, (like.dtype,), 2, like.device, "[rows, width]")
+    if t.shape != like.shape:
+        _reject(f"{name} shape {tuple(t.shape)} must equal {source_name}'s {tuple(like.shape)}", field=name,
+                value=tuple(t.shape), supported=tuple(like.shape))
+    _check_table(name, t)
+    if _shares_storage(t, like) and (t.data_ptr() != like.data_ptr() or _row_stride(t) != _row_stride(like)):
+        _reject(f"{name} overlaps {source_name} at another address: it must be {source_name} itself or a distinct "
+                "allocation", field=name, value="overlaps", supported=f"{source_name} or a distinct allocation")
+
+
+def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_out, weights_out, lens_out, freed,
+                 freed_lens) -> None:
+    device = page_table.device if isinstance(page_table, torch.Tensor) else None
+    _need("page_table", page_table, _INDEX, 2, device, "[rows, width]")
+    _check_table("page_table", page_table)
+    _need("weights", weights, (torch.float32,), 2, device, "[rows, >= width]")
+    _check_table("weights", weights)
+    width = page_table.shape[1]
+    if weights.shape[0] != page_table.shape[0] or weights.shape[1] < width:
+        _reject(f"weights shape {tuple(weights.shape)} must cover the page table's {tuple(page_table.shape)}",
+                field="weights", value=tuple(weights.shape), supported=tuple(page_table.shape))
+    _need("kv_lens", kv_lens, _INDEX, 1, device, "[batch]")
+    batch = kv_lens.shape[0]
+    if batch < 1:
+        _reject("kv_lens must hold at least one request", field="kv_lens", value=0, supported=">= 1")
+    _check_batch_vector("kv_lens", kv_lens, batch, device)
+    if rows is not None:
+        _check_batch_vector("rows", rows, batch, device)
+    elif page_table.shape[0] < batch:
+        _reject(f"page_table has {page_table.shape[0]} rows for a batch of {batch}", field="page_table",
+                value=int(page_table.shape[0]), supported=f">= {batch}")
+    for name, value, low in (("keep", keep, 1), ("protect_first", first, 0), ("protect_last", last, 0)):
+        if isinstance(value, bool) or not isinstance(value, int) or not low <= value < 1 << 31:
+            _reject(f"{name} must be an int >= {low}, got {value!r}", field=name, value=value, supported=f">= {low}")
+    if first + last > keep:
+        _reject(f"protect_first={first} and protect_last={last} exceed keep={keep}", field="keep", value=keep,
+                supported=f">= {first + last}")
+    _check_out("page_table_out", table_out, page_table, "page_table")
+    _check_out("weights_out", weights_out, weights, "weights")
+    if lens_out is not kv_lens:
+        _check_batch_vector("kv_lens_out", lens_out, batch, device)
+        if lens_out.dtype != kv_lens.dtype:
+            _reject(f"kv_lens_out dtype {_dtype_name(lens_out.dtype)} must equal kv_lens dtype "
+                    f"{_dtype_name(kv_lens.dtype)}", field="kv_lens_out", value=_dtype_name(lens_out.dtype),
+                    supported=_dtype_name(kv_lens.dtype))
+        if _shares_storage(lens_out, kv_lens) and lens_out.data_ptr() != kv_lens.data_ptr():
+            _reject("kv_lens_out overlaps kv_lens at another address", field="kv_lens_out", value="overlaps",
+                    supported="kv_lens or a distinct allocation")
+    if freed is not None:
+        _need("freed", freed, (page_table.dtype,), 2, device, "[batch, >= width - keep]")
+        if freed.shape[0] != batch or freed.shape[1] < max(1, width - keep):
+            _reject(f"freed shape {tuple(freed.shape)} must be at least {(batch, max(1, width - keep))}", field="freed",
+                    value=tuple(freed.shape), supported=(batch, max(1, width - keep)))
+        _check_table("freed", freed)
+        if _shares_storage(freed, page_table) or _shares_storage(freed, table_out):
+            _reject("freed must not overlap the page table", field="freed", value="overlaps",
+                    supported="a distinct allocation")
+    if freed_lens is not None:
+        _need("freed_lens", freed_lens, (torch.int32,), 1, device, "[batch]")
+        _check_batch_vector("freed_lens", freed_lens, batch, device)
+        if _shares_storage(freed_lens, kv_lens) or _shares_storage(freed_lens, lens_out):
+            _reject("freed_lens must not overlap kv_lens", field="freed_lens", value="overlaps",
+                    supported="a distinct allocation")
+
+
+def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: int = 0, protect_last: int = 0, rows=None,
+                   page_table_out=None, weights_out=None, kv_lens_out=None, freed=None, freed_lens=None):
+    """Shorten every request of more than `keep` positions to `keep`, by accumulated weight.
+
+    `page_table` [rows, width] int32 or int64, `weights` [rows, >= width] FP32, `kv_lens` [batch] and
+    `rows` [batch] int32 or int64 as in `paged_decode`.  The first `protect_first` and the last
+    `protect_last` positions of a request stay; of the others the heaviest stay (NaN counts as -inf; of
+    equal weights the lowest positions stay).  What stays moves to the front of its row in position
+    order, slots and weights alike; the weights behind it, up to the old length, become 0; table entries
+    behind it are left as they were.  A shorter request keeps its row.  Requests must name distinct rows.
+
+    By default `page_table`, `weights` and `kv_lens` are changed in place; `page_table_out`,
+    `weights_out` and `kv_lens_out` of the same shapes take the result instead (other rows, and what lies
+    behind a request's old length, stay as they are).  `freed` [batch, >= width - keep] receives the
+    slots that go, in position order, and `freed_lens` [batch] int32 their number; both are allocated
+    when not given.  Enqueues on the current stream and does not synchronise.
+
+    Returns (page_table_out, weights_out, kv_lens_out, freed, freed_lens)."""
+    table_out = page_table if page_table_out is None else page_table_out
+    acc_out = weights if weights_out is None else weights_out
+    lens_out = kv_lens if kv_lens_out is None else kv_lens_out
+    _check_evict(page_table, weights, kv_lens, keep, protect_first, protect_last, rows, table_out, acc_out, lens_out,
+                 freed, freed_lens)
+    device = page_table.device
+    _need_cuda("evict_lightest", device)
+    from . import kernel
+
+    lib = kernel.load()
+    batch, (table_rows, width) = kv_lens.shape[0], page_table.shape
+    if freed is None:
+        freed = torch.empty((batch, max(1, width - keep)), dtype=page_table.dtype, device=device)
+    if freed_lens is None:
+        freed_lens = torch.empty(batch, dtype=torch.int32, device=device)
+    call = kernel.Evict(
+        page_table.data_ptr(), weights.data_ptr(), None if rows is None else rows.data_ptr(), kv_lens.data_ptr(),
+        table_out.data_ptr(), acc_out.data_ptr(), lens_out.data_ptr(), freed.data_ptr(), freed_lens.data_ptr(),
+        _row_stride(page_table), _row_stride(weights), _row_stride(table_out), _row_stride(acc_out), _row_stride(freed),
+        batch, table_rows, width, freed.shape[1], keep, protect_first, protect_last, _INDEX[page_table.dtype],
+        0 if rows is None else _INDEX[rows.dtype], _INDEX[kv_lens.dtype])
+    _call(device, lib.akl_evict_lightest, "akl_evict_lightest", call)
+    return table_out, acc_out, lens_out, freed, freed_lens

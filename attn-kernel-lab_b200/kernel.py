@@ -26,7 +26,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 
 #: Explicit -gencode, never a bare -arch: tcgen05 needs the arch-specific target.
 GENCODE = "arch=compute_100a,code=sm_100a"
-SOURCES = ("akl_prep.cu", "akl_attn_sm100.cu", "akl_merge.cu", "akl_api.cu", "akl_static_scratch.cu")
+SOURCES = ("akl_prep.cu", "akl_attn_sm100.cu", "akl_merge.cu", "akl_api.cu", "akl_static_scratch.cu",
+           "akl_decode.cu", "akl_weights.cu", "akl_evict.cu")
 #: Per-file extra flags.  The preprocessing kernels decide quantised bytes, so no
 #: multiply-add may be contracted there.
 EXTRA_FLAGS = {"akl_prep.cu": ("-fmad=false",)}
@@ -38,6 +39,7 @@ EXPORTS = (
     "akl_merge_states", "akl_prefill_extend_static_scratch",
     "akl_batch_layout", "akl_batch_plan", "akl_prefill_extend_batch", "akl_prefill_extend_batch_phases",
     "akl_selftest_exact_division", "akl_static_scratch_status",
+    "akl_decode_layout", "akl_paged_decode", "akl_weights_layout", "akl_extend_weights", "akl_evict_lightest",
 )
 
 AKL_OK = 0
@@ -111,6 +113,58 @@ class Batch(ctypes.Structure):
                 ("table", ctypes.c_void_p), ("table_bytes", ctypes.c_uint64),
                 ("kv_dtype", ctypes.c_int32), ("idx_dtype", ctypes.c_int32),
                 ("flags", ctypes.c_uint32), ("sm_scale", ctypes.c_float)]
+
+
+def _fields(spec: str):
+    """ctypes fields from lines of "type: names"."""
+    kinds = {"ptr": ctypes.c_void_p, "i32": ctypes.c_int32, "i64": ctypes.c_int64, "u64": ctypes.c_uint64,
+             "f32": ctypes.c_float}
+    out = []
+    for line in spec.strip().splitlines():
+        kind, names = line.split(":")
+        out += [(name, kinds[kind.strip()]) for name in names.split()]
+    return out
+
+
+class DecodePlan(ctypes.Structure):
+    _fields_ = _fields("""i32: max_requests q_heads kv_heads reserved_
+                          i64: max_weight_tokens""")
+
+
+class DecodeLayout(ctypes.Structure):
+    _fields_ = _fields("u64: total_bytes off_status off_parts off_lse off_scores")
+
+
+class Decode(ctypes.Structure):
+    _fields_ = (_fields("""ptr: q k_pool v_pool page_table rows kv_lens out lse_out weights workspace
+                           u64: workspace_bytes""")
+                + [("plan", DecodePlan)]
+                + _fields("""i64: pool_rows q_stride k_stride v_stride table_stride weights_stride
+                             i32: batch q_heads kv_heads table_rows table_width kv_dtype idx_dtype rows_dtype lens_dtype
+                             f32: sm_scale weight_decay"""))
+
+
+class WeightsPlan(ctypes.Structure):
+    _fields_ = _fields("i32: max_kv_len max_q_len q_heads kv_heads")
+
+
+class WeightsLayout(ctypes.Structure):
+    _fields_ = _fields("u64: total_bytes off_status off_q off_rows off_parts")
+
+
+class Weights(ctypes.Structure):
+    _fields_ = (_fields("""ptr: q k_pool idx lse weights workspace
+                           u64: workspace_bytes""")
+                + [("plan", WeightsPlan)]
+                + _fields("""i64: pool_rows q_stride k_stride
+                             i32: T N prefix q_heads kv_heads kv_dtype idx_dtype
+                             f32: sm_scale weight_decay"""))
+
+
+class Evict(ctypes.Structure):
+    _fields_ = _fields("""ptr: page_table weights rows kv_lens page_table_out weights_out kv_lens_out freed freed_lens
+                          i64: table_stride weights_stride table_out_stride weights_out_stride freed_stride
+                          i32: batch table_rows table_width freed_width keep first last idx_dtype rows_dtype lens_dtype""")
 
 
 class NativeError(RuntimeError):
@@ -222,6 +276,14 @@ def load():
         lib.akl_selftest_exact_division.restype = ctypes.c_int
         lib.akl_static_scratch_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.akl_static_scratch_status.restype = ctypes.c_int
+        for name, struct in (("akl_decode_layout", (DecodePlan, DecodeLayout)),
+                             ("akl_weights_layout", (WeightsPlan, WeightsLayout))):
+            getattr(lib, name).argtypes = [ctypes.POINTER(struct[0]), ctypes.POINTER(struct[1])]
+            getattr(lib, name).restype = ctypes.c_int
+        for name, struct in (("akl_paged_decode", Decode), ("akl_extend_weights", Weights),
+                             ("akl_evict_lightest", Evict)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
 

@@ -281,6 +281,120 @@ int akl_prefill_extend_static_scratch(const akl_call_t* call, void* stream);
  * point may be used on a device after cudaDeviceReset.  No counterpart in the reference. */
 int akl_static_scratch_status(int32_t* host_out, void* stream);
 
+/* ---- decode: one new token per request over the same pool ---------------------------------
+ * No counterpart in the reference, whose operator is the extend alone.  For request b with
+ * n = kv_lens[b] cached positions (its own new token's included, already written to the pool):
+ *   x[h][i]  = sm_scale log2e <q[b][h], K[slot(i)][h / group]>,  i < n
+ *   lse[b][h] = log2 sum_i 2^x[h][i];   out[b][h] = sum_i 2^(x[h][i] - lse[b][h]) V[slot(i)][h / group]
+ *   weights[row][i] = decay weights[row][i] + sum_h 2^(x[h][i] - lse[b][h])            (optional)
+ * with slot(i) = page_table[row][i], row = rows[b] (b itself when rows is NULL).  Lengths, rows and
+ * slots are read on the device, so a captured launch follows them.  n is cut to the table's width; a
+ * request with n <= 0 or a row outside the table gives out = 0, lse = -inf; a slot outside the pool is
+ * skipped.  With weights, no two requests of a call may name the same row. */
+typedef struct akl_decode_plan {
+  int32_t max_requests;
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t reserved_;
+  int64_t max_weight_tokens;  /* sum over a batch of the lengths, each rounded up to 64; 0: no weights */
+} akl_decode_plan_t;
+
+typedef struct akl_decode_layout {
+  uint64_t total_bytes;       /* 1024-byte aligned base */
+  uint64_t off_status;        /* [64] i32; word 0 = first device error code: AKL_ERR_TIMEOUT, or
+                               * AKL_ERR_CAPACITY when the lengths exceed max_weight_tokens (out and
+                               * lse are whole then, weights of the last requests are not updated) */
+  uint64_t off_parts;         /* partial states of requests that several CTAs share */
+  uint64_t off_lse;           /* [max_requests][Hq] f32 */
+  uint64_t off_scores;        /* x, f32, by 64-position chunk of the packed requests: [chunk][Hq][64] */
+} akl_decode_layout_t;
+
+typedef struct akl_decode {
+  const void* q;              /* [batch][Hq][256] bf16; q_stride elements from request to request */
+  const void* k_pool;         /* [pool_rows][Hkv][256] bf16 | fp16; row strides in elements */
+  const void* v_pool;
+  const void* page_table;     /* [table_rows][table_width] i64 | i32; table_stride entries per row */
+  const void* rows;           /* [batch] i64 | i32 or NULL */
+  const void* kv_lens;        /* [batch] i64 | i32 */
+  void* out;                  /* [batch][Hq][256] bf16 */
+  float* lse_out;             /* [batch][Hq] f32 base-2, or NULL */
+  float* weights;             /* [table_rows][>= table_width] f32, weights_stride per row, or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+  akl_decode_plan_t plan;
+  int64_t pool_rows, q_stride, k_stride, v_stride, table_stride, weights_stride;
+  int32_t batch, q_heads, kv_heads, table_rows, table_width;
+  int32_t kv_dtype;           /* AKL_KV_* */
+  int32_t idx_dtype, rows_dtype, lens_dtype;   /* AKL_IDX_* */
+  float sm_scale;
+  float weight_decay;         /* 0: weights are overwritten without being read */
+} akl_decode_t;
+
+int akl_decode_layout(const akl_decode_plan_t* plan, akl_decode_layout_t* out);
+int akl_paged_decode(const akl_decode_t* call, void* stream);
+
+/* ---- attention weights of an extend ----------------------------------------------------------
+ * What the T query rows of an extend (or its last T rows) attend to, summed over rows and q heads:
+ *   weights[i] = decay weights[i] + sum_{t, h: i <= prefix + t} 2^(sm_scale log2e <q[t][h], K[idx[i]][h / group]> - lse[t][h])
+ * lse is what akl_prefill_extend writes (base 2); a row whose lse is -inf or +inf adds nothing.
+ * No counterpart in the reference. */
+typedef struct akl_weights_plan {
+  int32_t max_kv_len, max_q_len, q_heads, kv_heads;
+} akl_weights_plan_t;
+
+typedef struct akl_weights_layout {
+  uint64_t total_bytes;       /* 1024-byte aligned base */
+  uint64_t off_status;        /* [64] i32; word 0 = AKL_ERR_TIMEOUT if a bounded wait ran out */
+  uint64_t off_q;             /* Q rows packed by kv head, in the pool's type */
+  uint64_t off_rows;          /* per packed row {factor, lse} f32 */
+  uint64_t off_parts;         /* [parts][max_kv_len] f32 partial sums */
+} akl_weights_layout_t;
+
+typedef struct akl_weights {
+  const void* q;              /* [T][Hq][256] bf16, q_stride elements from row to row */
+  const void* k_pool;         /* [pool_rows][Hkv][256] bf16 | fp16, k_stride elements per row */
+  const void* idx;            /* [N] i64 | i32; a slot outside the pool gets no weight */
+  const float* lse;           /* [T][Hq] */
+  float* weights;             /* [N] */
+  void* workspace;
+  uint64_t workspace_bytes;
+  akl_weights_plan_t plan;
+  int64_t pool_rows, q_stride, k_stride;
+  int32_t T, N, prefix, q_heads, kv_heads;
+  int32_t kv_dtype, idx_dtype;
+  float sm_scale;
+  float weight_decay;         /* 0: weights are overwritten without being read */
+} akl_weights_t;
+
+int akl_weights_layout(const akl_weights_plan_t* plan, akl_weights_layout_t* out);
+int akl_extend_weights(const akl_weights_t* call, void* stream);
+
+/* ---- eviction by accumulated weight ------------------------------------------------------------
+ * For each request with more than `keep` positions: its first `first` and last `last` positions stay,
+ * and of the others the keep - first - last heaviest (NaN counts as -inf; of equal weights the lowest
+ * positions stay).  Staying slots and weights move to the front of the row in position order, the
+ * weights behind them up to the old length become 0, the slots that go are listed in `freed` in
+ * position order.  Table entries behind the new length, and freed entries behind the count, are left
+ * as they were.  The outputs may be the inputs themselves (same address and stride).  No two requests
+ * may name the same row.  No counterpart in the reference. */
+typedef struct akl_evict {
+  const void* page_table;     /* [table_rows][table_width] i64 | i32 */
+  const float* weights;       /* [table_rows][>= table_width] */
+  const void* rows;           /* [batch] or NULL */
+  const void* kv_lens;        /* [batch] */
+  void* page_table_out;
+  float* weights_out;
+  void* kv_lens_out;          /* [batch], type of kv_lens; may be kv_lens */
+  void* freed;                /* [batch][freed_width], type of the table; freed_width >= table_width - keep */
+  int32_t* freed_lens;        /* [batch] */
+  int64_t table_stride, weights_stride, table_out_stride, weights_out_stride, freed_stride;
+  int32_t batch, table_rows, table_width, freed_width;
+  int32_t keep, first, last;
+  int32_t idx_dtype, rows_dtype, lens_dtype;
+} akl_evict_t;
+
+int akl_evict_lightest(const akl_evict_t* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
