@@ -1,6 +1,34 @@
 // Decode attention: one new token per request over the paged pool.
 //   x = c <q, k>, c = sm_scale log2 e;  m = max x;  l = sum 2^(x - m);  out = sum 2^(x - m) v / l;
-//   lse = m + log2 l;   weights += sum over the q heads of 2^(x - lse)
+//   lse = m + log2 l;   weights (+)= sum over the q heads of 2^(x - lse)
+//
+// K and V are read once, 1 KiB per position and kv head for 4 * 256 * group operations: HBM bound for
+// every group up to 8.  So the kernel is a copy pipeline with arithmetic that keeps out of its way:
+//
+//   * one CTA per SM; the positions of all requests, cut into tiles of 64 KiB of K and V, form one
+//     sequence of which every CTA takes an equal share, whatever the lengths (they are read here, on
+//     the device).  A CTA meets a run of requests: those it holds whole it finishes itself, of the
+//     first and the last it may hold a part, whose (m, l, unnormalised out) goes to the workspace for
+//     the join launch.  No atomics: partial states are joined in position order.
+//   * a producer warp gathers the rows by bulk copies, one per position and plane (the kv heads of a
+//     position are neighbours in the pool: 2 KiB at four heads), into a ring of three tiles, with the
+//     page-table entries three tiles ahead.  Rows lie 16 bytes off a multiple of 128 in shared memory,
+//     so that matrix loads meet no bank twice.
+//   * eight warps: four (kv head, 16 positions) tasks times two halves of the output channels.  Both
+//     halves form the scores, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
+//     heads of the kv head on N -- with the heads on M half to three quarters of the tensor work would
+//     be padding.  Out^T = V^T P^T takes P^T in the operand layout that an 8x8 transpose of the score
+//     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: a tile needs 8192
+//     multiply-adds per position and kv head against the ~43 cycles that its bytes take per SM, an eighth of
+//     the mma.sync rate; tcgen05's 128 rows would be 6 to 25 % filled and its TMEM round trip longer.
+//
+// Rounding: scores, m, l and both sums are 32-bit.  P enters the second product as two 16-bit parts,
+// p = hi + lo (2^-16 relative): with one part alone the output error was 1.2 times that of the BF16
+// rounding of the result, and the extra products are free here.  For an FP16 pool P is scaled by 2^14, so
+// that small probabilities stay normal numbers, and Q (BF16) is brought to FP16 by the power of two
+// of its row's largest element: exact down to 2^-17 of that element, 2^-25 of it below.
+#include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "akl_common.cuh"
@@ -10,139 +38,710 @@ namespace akl {
 
 namespace {
 
+using namespace ptx;
+
 constexpr int kChunk = 64;          // positions per chunk of recorded scores
 constexpr int kMaxGroup = 8;        // query heads per kv head
+constexpr int kMaxCtas = 160;       // CTAs whose partial states the workspace holds (two each)
+constexpr int kStages = 3;
+constexpr int kWarps = 8;           // consumers; one more warp produces
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kMinTiles = 1;        // tiles a CTA takes at least
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr long long kWaitCycles = 4000000000ll;      // ~2 s: a wait that long is a defect
 
 inline uint64_t align1k(uint64_t x) { return (x + 1023) / 1024 * 1024; }
+
+// Heads per CTA and what follows from them.
+template <int HB>
+struct Tile {
+  static constexpr int kRow = HB * 512;              // bytes of one position's heads in one plane
+  static constexpr int kPitch = kRow + 16;
+  static constexpr int kPos = 64 / HB;               // positions per tile
+  static constexpr int kPlane = kPos * kPitch;
+  static constexpr int kStage = 2 * kPlane;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kGroups = 4 / HB;             // 16-position groups of a tile
+  static constexpr int kMerge = kGroups > 1 ? 16384 : 0;
+  static constexpr int kOffMerge = kRing;
+  static constexpr int kOffMl = kOffMerge + kMerge;  // [8 warps][8 heads] {m, l}
+  static constexpr int kOffMask = kOffMl + 512;      // [kStages] u64: positions of the tile that are there
+  static constexpr int kOffBar = kOffMask + 8 * kStages;
+  static constexpr int kSmem = kOffBar + 16 * kStages + 16;
+};
+static_assert(Tile<1>::kSmem <= 232448 && Tile<2>::kSmem <= 232448 && Tile<4>::kSmem <= 232448, "shared memory");
+
+// Workspace, behind off_parts: who holds which request, then the partial states.
+constexpr int kSlotHeads = 4 * kMaxGroup;
+inline uint64_t info_bytes(const akl_decode_plan_t& p) { return align1k(static_cast<uint64_t>(p.max_requests) * 2 * 16); }
+constexpr uint64_t kMlBytes = static_cast<uint64_t>(2 * kMaxCtas) * kSlotHeads * 8;
+constexpr uint64_t kPartBytes = static_cast<uint64_t>(2 * kMaxCtas) * kSlotHeads * 1024;
 
 int decode_layout(const akl_decode_plan_t& p, akl_decode_layout_t* o) {
   if (p.max_requests < 1 || p.q_heads < 1 || p.kv_heads < 1 || p.max_weight_tokens < 0) return AKL_ERR_INVALID;
   if (p.q_heads % p.kv_heads || p.q_heads / p.kv_heads > kMaxGroup) return AKL_ERR_UNSUPPORTED;
   std::memset(o, 0, sizeof(*o));
-  uint64_t off = 0;
-  o->off_status = off;
-  off += 1024;
+  uint64_t off = 1024;
   o->off_parts = off;
+  off += info_bytes(p) + align1k(kMlBytes) + kPartBytes;
   o->off_lse = off;
   off += align1k(static_cast<uint64_t>(p.max_requests) * p.q_heads * 4);
   o->off_scores = off;
+  off += align1k((static_cast<uint64_t>(p.max_weight_tokens) + kChunk - 1) / kChunk * kChunk * p.q_heads * 4);
   o->total_bytes = off;
   return AKL_OK;
 }
 
-__device__ __forceinline__ void request_of(const akl_decode_t& c, int b, long long& row, int& n) {
+// What the kernels get besides the call.
+struct Work {
+  int* status;
+  int4* info;            // [request][head block] {first slot, first CTA, last CTA, -}
+  float2* ml;            // [slot][kSlotHeads]
+  float* parts;          // [slot][kSlotHeads][256]
+  float* lse;            // [batch][Hq], for the weights
+  float* scores;         // [chunk][Hq][64] or NULL
+  long long max_chunks;
+};
+
+// Cached positions of request b and its table row; 0 where there is nothing to read.
+__device__ __forceinline__ int request_of(const akl_decode_t& c, int b, long long& row) {
   row = c.rows != nullptr ? load_index(c.rows, c.rows_dtype, b) : b;
   long long len = load_index(c.kv_lens, c.lens_dtype, b);
   len = len < 0 ? 0 : (len > c.table_width ? c.table_width : len);
   if (row < 0 || row >= c.table_rows) { row = 0; len = 0; }
-  n = static_cast<int>(len);
+  return static_cast<int>(len);
 }
 
-// One CTA per (request, kv head); a warp takes every eighth position, a lane eight channels.
-template <int KV>
-__global__ void __launch_bounds__(256) decode_kernel(akl_decode_t c, float* lse_ws) {
-  __shared__ float sm_m[8][kMaxGroup], sm_l[8][kMaxGroup];
-  __shared__ float sm_o[8][256];
-  const int b = blockIdx.x, j = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = c.q_heads / c.kv_heads;
-  long long row;
-  int n;
-  request_of(c, b, row, n);
-  float q[kMaxGroup][8], o[kMaxGroup][8], m[kMaxGroup], l[kMaxGroup];
+__device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
-  for (int h = 0; h < kMaxGroup; ++h) {
-    m[h] = -INFINITY;
-    l[h] = 0.f;
-    if (h < group) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + b * c.q_stride + (j * group + h) * 256 + lane * 8);
-      unpack8<AKL_KV_BF16>(raw, q[h]);
+  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  return v;
+}
+
+// A warp's place in the sequence of tiles: request b, head block hb, tile t of nt.  The lengths of 32
+// requests at a time are spread over the lanes.
+template <int HB>
+struct Cursor {
+  static constexpr int kPos = Tile<HB>::kPos;
+  const akl_decode_t& c;
+  const int lane, blocks;           // head blocks
+  int base, lane_n;
+  long long lane_row;
+  int b, n, nt, hb, t;
+  long long row, chunk0;            // chunk0: score chunks of the requests before b
+
+  __device__ __forceinline__ Cursor(const akl_decode_t& call, int l) : c(call), lane(l), blocks(call.kv_heads / HB) {}
+
+  __device__ __forceinline__ long long total() const {
+    long long tiles = 0;
+#pragma unroll 4
+    for (int i = lane; i < c.batch; i += 32) {
+      long long r;
+      tiles += (request_of(c, i, r) + kPos - 1) / kPos;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[h][i] = h < group ? q[h][i] * (c.sm_scale * kLog2e) : 0.f;
-      o[h][i] = 0.f;
-    }
+    return warp_sum(tiles) * blocks;
   }
-  for (int i = warp; i < n; i += 8) {
-    const long long slot = load_index(c.page_table, c.idx_dtype, row * c.table_stride + i);
-    if (slot < 0 || slot >= c.pool_rows) continue;
-    float k[8], v[8];
-    unpack8<KV>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + j * 256 + lane * 8), k);
-    unpack8<KV>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.v_pool) + slot * c.v_stride + j * 256 + lane * 8), v);
-#pragma unroll
-    for (int h = 0; h < kMaxGroup; ++h) {
-      if (h >= group) break;
-      float x = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x = fmaf(q[h][e], k[e], x);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-      const float top = fmaxf(m[h], x), a = exp2f(m[h] - top), p = exp2f(x - top);
-      m[h] = top;
-      l[h] = l[h] * a + p;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[h][e] = fmaf(p, v[e], o[h][e] * a);
-    }
+  __device__ __forceinline__ void window(int at) {
+    base = at;
+    lane_n = 0;
+    lane_row = 0;
+    if (at + lane < c.batch) lane_n = request_of(c, at + lane, lane_row);
   }
-  for (int h = 0; h < group; ++h) {
-    float mh = 0.f, lh = 0.f;
+  __device__ __forceinline__ void take(int i) {
+    b = base + i;
+    n = __shfl_sync(0xffffffffu, lane_n, i);
+    row = __shfl_sync(0xffffffffu, lane_row, i);
+    nt = (n + kPos - 1) / kPos;
+  }
+  // Tile `at` of the sequence; there is one.
+  __device__ __forceinline__ void seek(long long at) {
+    chunk0 = 0;
+    for (window(0);; window(base + 32)) {
+      const int tiles = (lane_n + kPos - 1) / kPos * blocks;
+      long long upto = tiles;
 #pragma unroll
-    for (int k = 0; k < kMaxGroup; ++k)
-      if (k == h) { mh = m[k]; lh = l[k]; }
-    if (lane == 0) { sm_m[warp][h] = mh; sm_l[warp][h] = lh; }
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, sm_l[w][h] != 0.f ? sm_m[w][h] : -INFINITY);
-    for (int w = 0; w < 8; ++w) total += sm_l[w][h] != 0.f ? sm_l[w][h] * exp2f(sm_m[w][h] - top) : 0.f;
-    const float f = lh != 0.f ? exp2f(mh - top) : 0.f;
-#pragma unroll
-    for (int k = 0; k < kMaxGroup; ++k)
-      if (k == h) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sm_o[warp][lane * 8 + e] = lh != 0.f ? o[k][e] * f : 0.f;
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += v;
       }
-    __syncthreads();
-    float sum = 0.f;
-    for (int w = 0; w < 8; ++w) sum += sm_o[w][threadIdx.x];
-    const int head = j * group + h;
-    const bool none = total == 0.f;
-    reinterpret_cast<__nv_bfloat16*>(c.out)[(static_cast<long long>(b) * c.q_heads + head) * 256 + threadIdx.x] =
-        __float2bfloat16_rn(none ? 0.f : sum / total);
-    if (threadIdx.x == 0) {
-      const float lse = none ? -INFINITY : top + log2f(total);
-      if (c.lse_out != nullptr) c.lse_out[b * c.q_heads + head] = lse;
-      lse_ws[b * c.q_heads + head] = lse;
+      const unsigned past = __ballot_sync(0xffffffffu, upto > at);
+      const int chunks = (lane_n + kChunk - 1) / kChunk;
+      if (past != 0u) {
+        const int i = __ffs(past) - 1;
+        take(i);
+        const int in = static_cast<int>(at - __shfl_sync(0xffffffffu, upto - tiles, i));
+        hb = in / nt;
+        t = in - hb * nt;
+        chunk0 += warp_sum(lane < i ? chunks : 0);
+        return;
+      }
+      at -= __shfl_sync(0xffffffffu, upto, 31);
+      chunk0 += warp_sum(chunks);
+      if (base + 32 >= c.batch) { b = c.batch; n = nt = hb = t = 0; return; }   // not reached
     }
-    __syncthreads();
+  }
+  // On to the next tile; only where there is one.
+  __device__ __forceinline__ void next() {
+    if (++t < nt) return;
+    t = 0;
+    if (++hb < blocks) return;
+    hb = 0;
+    do {
+      chunk0 += (n + kChunk - 1) / kChunk;
+      if (b + 1 >= c.batch) { n = nt = 0; return; }                            // not reached
+      if (b + 1 == base + 32) window(base + 32);
+      take(b + 1 - base);
+    } while (n == 0);
+  }
+};
+
+struct Wait {
+  int* status;
+  volatile int* aborted;   // shared memory
+  // Every waiter observes every phase of its barriers in order.  False after ~2 s, or once another
+  // thread of the CTA gave up; the status word then says so.
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    if (mbar_try_wait(bar, parity)) return true;
+    long long t0 = 0;
+    for (uint32_t spin = 1;; ++spin) {
+      if (mbar_try_wait(bar, parity)) return true;
+      if ((spin & 0x3FFu) == 0) {
+        if (t0 == 0) t0 = clock64();
+        if (*aborted || clock64() - t0 > kWaitCycles) {
+          *aborted = 1;
+          atomicCAS(status, 0, AKL_ERR_TIMEOUT);
+          return false;
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// D[16 x 8] += A[16 x 16] B[16 x 8], 16-bit operands of the pool's type, 32-bit sums.
+template <int KV>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (KV == AKL_KV_BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two floats to the pool's type, and what that rounding left of them.
+template <int KV>
+__device__ __forceinline__ uint32_t split2(float a, float b, uint32_t& rest) {
+  uint32_t hi;
+  if (KV == AKL_KV_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    rest = *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    rest = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return hi;
+}
+
+// Queries of one kv head as the B operand: thread (g, q) = (lane / 4, lane % 4) holds head g, channels
+// 16 k + 2 q, + 1 and the same + 8.  cs: what scores of the heads 2 q and 2 q + 1 are multiplied by.
+template <int KV>
+__device__ __forceinline__ void load_q(const akl_decode_t& c, int b, int head0, int group, int lane, uint32_t (&q)[16][2], float (&cs)[2]) {
+  const int g = lane >> 2, quad = lane & 3;
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(c.q) + b * c.q_stride + (head0 + g) * 256) + quad;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    q[k][0] = g < group ? __ldg(src + k * 8) : 0u;
+    q[k][1] = g < group ? __ldg(src + k * 8 + 4) : 0u;
+  }
+  cs[0] = cs[1] = c.sm_scale * kLog2e;
+  if (KV == AKL_KV_FP16) {
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        top = fmaxf(top, fmaxf(fabsf(bf16_bits_to_float(q[k][e] & 0xFFFFu)), fabsf(bf16_bits_to_float(q[k][e] >> 16))));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e <= top < 2^(e+1), with both 2^e and 2^-e normal; 1 for a row of zeros or of infinities
+    int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xFFu) - 127;
+    e = (top == 0.f || e == 128) ? 0 : max(-126, min(126, e));
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const __half2 h = __floats2half2_rn(bf16_bits_to_float(q[k][i] & 0xFFFFu) * down, bf16_bits_to_float(q[k][i] >> 16) * down);
+        q[k][i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    cs[0] *= __shfl_sync(0xffffffffu, up, quad * 8);
+    cs[1] *= __shfl_sync(0xffffffffu, up, quad * 8 + 4);
   }
 }
 
-// One warp per position.
-template <int KV>
-__global__ void __launch_bounds__(256) decode_weights_kernel(akl_decode_t c, const float* lse_ws) {
-  const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
+// Producer: the rows of every tile of this CTA's share.
+template <int HB>
+__device__ __forceinline__ void produce(const akl_decode_t& c, uint32_t smem, uint8_t* smem_gen, const Wait& wait,
+                                        Cursor<HB>& at, long long first, int count, int lane) {
+  using T = Tile<HB>;
+  constexpr int kPairs = T::kPos / 16;               // (position, plane) pairs per lane
+  constexpr int kSlots = T::kPos > 32 ? 2 : 1;       // positions per lane
+  long long slot[kStages][kSlots];
+  int block[kStages];
+  // page-table entries of the tile the cursor is at; -1: nothing to read
+  auto look = [&](long long (&s)[kSlots], int& hb) {
+    hb = at.hb;
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+      const int i = at.t * T::kPos + (lane + 32 * k) % T::kPos;
+      s[k] = -1;
+      if (i < at.n) {
+        s[k] = load_index(c.page_table, c.idx_dtype, at.row * c.table_stride + i);
+        if (s[k] >= c.pool_rows) s[k] = -1;
+      }
+    }
+  };
+  at.seek(first);
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) {
+    if (s < count) {
+      if (s > 0) at.next();
+      look(slot[s], block[s]);
+    }
+  }
+  const uint32_t bars = smem + T::kOffBar;
+  int issued = 0;
+  for (int it = 0; it < count; ++it) {
+    const int st = it % kStages;
+    if (it >= kStages && (!wait(bars + (kStages + st) * 8, ((it / kStages) - 1) & 1) || *wait.aborted)) break;
+    long long now[kSlots];
+    int there = 0;
+    unsigned long long mask = 0;
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+      now[k] = slot[0][k];
+      const unsigned m = __ballot_sync(0xffffffffu, now[k] >= 0) & (T::kPos < 32 ? (1u << (T::kPos & 31)) - 1u : 0xffffffffu);
+      mask |= static_cast<unsigned long long>(m) << (32 * k);
+      there += __popc(m);
+    }
+    const long long head0 = static_cast<long long>(block[0]) * (HB * 256);
+    if (lane == 0) {
+      *reinterpret_cast<volatile unsigned long long*>(smem_gen + T::kOffMask + st * 8) = mask;
+      mbar_expect_tx(bars + st * 8, static_cast<uint32_t>(there) * (2u * T::kRow));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < kPairs; ++p) {
+      const int pair = lane + 32 * p, pos = pair % T::kPos, plane = pair / T::kPos;
+      const long long s = now[kSlots == 2 ? p & 1 : 0];
+      if (s >= 0) {
+        const uint16_t* src = plane == 0 ? static_cast<const uint16_t*>(c.k_pool) + s * c.k_stride + head0
+                                         : static_cast<const uint16_t*>(c.v_pool) + s * c.v_stride + head0;
+        bulk_g2s(smem + st * T::kStage + plane * T::kPlane + pos * T::kPitch, src, T::kRow, bars + st * 8);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s + 1 < kStages; ++s) {
+      block[s] = block[s + 1];
+#pragma unroll
+      for (int k = 0; k < kSlots; ++k) slot[s][k] = slot[s + 1][k];
+    }
+    if (it + kStages < count) {
+      at.next();
+      look(slot[kStages - 1], block[kStages - 1]);
+    }
+    issued = it + 1;
+  }
+  // no copy may outlive the CTA: they land (or the limit passes) before this warp ends
+  for (int it = issued > kStages ? issued - kStages : 0; it < issued; ++it) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bars + (it % kStages) * 8, (it / kStages) & 1) && clock64() - t0 < kWaitCycles) {}
+  }
+}
+
+template <int KV, int HB>
+__global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t c, const Work w) {
+  using T = Tile<HB>;
+  extern __shared__ __align__(128) uint8_t smem_gen[];
+  __shared__ int sm_aborted;
+  const uint32_t smem = smem_u32(smem_gen);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    sm_aborted = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem + T::kOffBar + i * 8, 1);
+      mbar_init(smem + T::kOffBar + (kStages + i) * 8, kWarps);
+    }
+    mbar_init_fence();
+  }
+  Cursor<HB> at(c, lane);
+  const long long total = at.total();
+  long long ctas = (total + kMinTiles - 1) / kMinTiles;
+  if (ctas > gridDim.x) ctas = gridDim.x;
+  if (blockIdx.x >= ctas) return;                    // the whole CTA: nothing waits for it
+  const long long first = total * blockIdx.x / ctas;
+  const int count = static_cast<int>(total * (blockIdx.x + 1) / ctas - first);
+  __syncthreads();
+  const Wait wait{w.status, &sm_aborted};
+
+  if (warp == kWarps) {
+    produce<HB>(c, smem, smem_gen, wait, at, first, count, lane);
+    return;
+  }
+
+  // ---- consumers: kv head `unit` of the block, positions 16 tg .. of the tile, channels 128 half ..
+  const int unit = (warp & 3) % HB, tg = (warp & 3) / HB, half = warp >> 2;
+  const int g = lane >> 2, quad = lane & 3, group = c.q_heads / c.kv_heads;
+  const uint32_t bars = smem + T::kOffBar;
+  constexpr float kShift = KV == AKL_KV_FP16 ? 14.f : 0.f;   // P carries 2^kShift
+  const uint32_t k_lane = (tg * 16 + (lane & 15)) * T::kPitch + unit * 512 + (lane >> 4) * 16;
+  const uint32_t v_lane = T::kPlane + (tg * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * T::kPitch + unit * 512 + half * 256 +
+                          ((lane >> 3) & 1) * 16;
+  uint32_t q[16][2];
+  float cs[2], m[2], l[2], o[8][4];
+  bool ok = true, new_piece = true;
+  int t_begin = 0;
+  at.seek(first);
+  for (int it = 0; it < count; ++it) {
+    if (new_piece) {
+      load_q<KV>(c, at.b, (at.hb * HB + unit) * group, group, lane, q, cs);
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      t_begin = at.t;
+      new_piece = false;
+    }
+    const int st = it % kStages;
+    const uint32_t stage = smem + st * T::kStage;
+    if (ok) ok = wait(bars + st * 8, (it / kStages) & 1);
+    if (ok) {
+      const unsigned there = static_cast<unsigned>(*reinterpret_cast<volatile unsigned long long*>(smem_gen + T::kOffMask + st * 8) >> (16 * tg)) & 0xFFFFu;
+      // scores of 16 positions x 8 heads: thread has positions g, g + 8 of heads 2 quad, 2 quad + 1.
+      // Four chains of four products keep the sums short, in time and in rounding.
+      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (there != 0u) {
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          uint32_t a[4];
+          ldsm4(stage + k_lane + k * 32, a);
+          mma16<KV>(s[k & 3], a, q[k][0], q[k][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ((s[0][i] + s[1][i]) + (s[2][i] + s[3][i])) * cs[i & 1];
+        if (there != 0xFFFFu) {
+          if (!((there >> g) & 1u)) x[0] = x[1] = -INFINITY;
+          if (!((there >> (g + 8)) & 1u)) x[2] = x[3] = -INFINITY;
+          // V rows that were not read hold anything: clear them (this warp's channels), for 0 * NaN is not 0.
+          // The next copy into them follows this warp's arrival, behind the proxy fence.
+          for (unsigned gone = ~there & 0xFFFFu; gone != 0u; gone &= gone - 1u) {
+            const uint32_t at_row = stage + T::kPlane + (tg * 16 + __ffs(gone) - 1) * T::kPitch + unit * 512 + half * 256;
+            if (lane < 16) st_shared_v4(at_row + lane * 16, 0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+      }
+      if (w.scores != nullptr && half == 0) {
+        const long long chunk = at.chunk0 + (at.t * T::kPos + tg * 16) / kChunk;
+        if (chunk < w.max_chunks) {
+          float* dst = w.scores + (chunk * c.q_heads + (at.hb * HB + unit) * group) * kChunk + (at.t * T::kPos + tg * 16) % kChunk + g;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (quad * 2 + e < group) {
+              dst[(quad * 2 + e) * kChunk] = x[e];
+              dst[(quad * 2 + e) * kChunk + 8] = x[e + 2];
+            }
+        }
+      }
+      if (there != 0u) {
+        float safe[2];
+        bool moved = false;
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(x[e], x[e + 2]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float m_new = fmaxf(m[e], top);
+          safe[e] = m_new == -INFINITY ? 0.f : m_new;      // nothing but scores of -inf so far: they weigh 0
+          alpha[e] = ex2(m[e] - safe[e]);
+          moved |= m_new != m[e];
+          m[e] = m_new;
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+          l[0] *= alpha[0];
+          l[1] *= alpha[1];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[i][0] *= alpha[0];
+            o[i][1] *= alpha[1];
+            o[i][2] *= alpha[0];
+            o[i][3] *= alpha[1];
+          }
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = ex2(x[i] - safe[i & 1] + kShift);
+          l[i & 1] += p[i];
+        }
+        uint32_t lo0, lo1;
+        uint32_t hi0 = split2<KV>(p[0], p[1], lo0), hi1 = split2<KV>(p[2], p[3], lo1);
+        hi0 = transpose8x8(hi0);
+        hi1 = transpose8x8(hi1);
+        lo0 = transpose8x8(lo0);
+        lo1 = transpose8x8(lo1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t a[4];
+          ldsm4_trans(stage + v_lane + i * 32, a);
+          mma16<KV>(o[i], a, hi0, hi1);
+          mma16<KV>(o[i], a, lo0, lo1);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars + (kStages + st) * 8);
+    if (at.t + 1 < at.nt && it + 1 < count) {
+      ++at.t;
+      continue;
+    }
+
+    // ---- end of this CTA's piece of (request, head block)
+    new_piece = true;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
+    }
+    if (!ok) {                        // a bounded wait ran out: leave nothing that looks like a result
+      l[0] = l[1] = __int_as_float(0x7FC00000);
+      m[0] = m[1] = 0.f;
+    }
+    if (T::kGroups > 1) {
+      // join the position groups of each kv head: a common maximum, then pairwise sums through shared memory
+      float2* ml = reinterpret_cast<float2*>(smem_gen + T::kOffMl);
+      float* buf = reinterpret_cast<float*>(smem_gen + T::kOffMerge);
+      if (g == 0) {
+        ml[warp * 8 + quad * 2] = make_float2(m[0], l[0]);
+        ml[warp * 8 + quad * 2 + 1] = make_float2(m[1], l[1]);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < T::kGroups; ++k) top = fmaxf(top, ml[(half * 4 + k * HB + unit) * 8 + quad * 2 + e].x);
+        const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < T::kGroups; ++k) {
+          const float2 v = ml[(half * 4 + k * HB + unit) * 8 + quad * 2 + e];
+          sum += v.y * ex2(v.x - safe);
+        }
+        const float f = ex2(m[e] - safe);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { o[i][e] *= f; o[i][e + 2] *= f; }
+        m[e] = top;
+        l[e] = sum;
+      }
+#pragma unroll
+      for (int step = T::kGroups / 2; step > 0; step >>= 1) {
+        // groups step .. 2 step - 1 hand theirs to groups 0 .. step - 1
+        const int pair = (half * step + (tg % step)) * HB + unit;       // at most 4 pairs of 4 KiB
+        if (tg >= step && tg < 2 * step) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) buf[(pair * 32 + i) * 32 + lane] = o[i >> 2][i & 3];
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tg < step) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i >> 2][i & 3] += buf[(pair * 32 + i) * 32 + lane];
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+    }
+    const bool whole = t_begin == 0 && at.t + 1 == at.nt;
+    const int piece_slot = 2 * blockIdx.x + (first + it - (at.t - t_begin) == first ? 0 : 1);
+    if (warp == 0 && lane == 0) {
+      int* info = reinterpret_cast<int*>(w.info + at.b * 2 + at.hb);
+      if (t_begin == 0) { info[0] = piece_slot; info[1] = blockIdx.x; }
+      if (at.t + 1 == at.nt) info[2] = blockIdx.x;
+    }
+    if (tg == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = quad * 2 + e;
+        if (h >= group) break;
+        const int head = (at.hb * HB + unit) * group + h;
+        if (whole) {
+          const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(c.out) + (static_cast<long long>(at.b) * c.q_heads + head) * 256 + half * 128 + g;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dst[i * 16] = __float2bfloat16_rn(o[i][e] * inv);
+            dst[i * 16 + 8] = __float2bfloat16_rn(o[i][e + 2] * inv);
+          }
+          if (half == 0 && g == 0) {
+            const float lse = l[e] == 0.f ? -INFINITY : m[e] + (log2f(l[e]) - kShift);
+            w.lse[static_cast<long long>(at.b) * c.q_heads + head] = lse;
+            if (c.lse_out != nullptr) c.lse_out[static_cast<long long>(at.b) * c.q_heads + head] = lse;
+          }
+        } else {
+          const int at_head = piece_slot * kSlotHeads + unit * group + h;
+          float* dst = w.parts + static_cast<long long>(at_head) * 256 + half * 128 + g;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dst[i * 16] = o[i][e];
+            dst[i * 16 + 8] = o[i][e + 2];
+          }
+          if (half == 0 && g == 0) w.ml[at_head] = make_float2(m[e] - kShift, l[e]);
+        }
+      }
+    }
+    if (it + 1 < count) at.next();
+  }
+}
+
+// Join of the partial states of one (request, q head): lse = log2 sum_i l_i 2^m_i, out = sum_i 2^(m_i - lse) O_i,
+// in position order.  A request without positions gets its zeros here.
+__global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, const Work w, int hb_heads) {
+  __shared__ float sm_f[kMaxCtas + 1];
+  __shared__ float sm_red[16];
+  __shared__ __align__(16) float sm_o[3][256];   // read and written as float4
+  const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long long row;
-  int n;
-  request_of(c, b, row, n);
-  for (int i = blockIdx.y * 8 + warp; i < n; i += gridDim.y * 8) {
-    const long long slot = load_index(c.page_table, c.idx_dtype, row * c.table_stride + i);
+  const int n = request_of(c, b, row);
+  const int hb = head / hb_heads, h = head - hb * hb_heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + (static_cast<long long>(b) * c.q_heads + head) * 256;
+  const long long at = static_cast<long long>(b) * c.q_heads + head;
+  if (n == 0) {
+    out[tid] = __float2bfloat16_rn(0.f);
+    if (tid == 0) {
+      w.lse[at] = -INFINITY;
+      if (c.lse_out != nullptr) c.lse_out[at] = -INFINITY;
+    }
+    return;
+  }
+  const int4 info = w.info[b * 2 + hb];
+  const int parts = info.z - info.y + 1;
+  if (parts == 1) return;                            // one CTA held the request and wrote the result
+  auto slot = [&](int i) { return i == 0 ? info.x : 2 * (info.y + i); };
+  float2 mine = make_float2(-INFINITY, 0.f);
+  if (tid < parts) mine = w.ml[slot(tid) * kSlotHeads + h];
+  float top = warp_max(mine.x);
+  if (lane == 0) sm_red[warp] = top;
+  __syncthreads();
+  top = sm_red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, sm_red[i]);
+  const float safe = top == -INFINITY ? 0.f : top;
+  const float f = ex2(mine.x - safe);
+  if (tid < parts) sm_f[tid] = f;
+  float sum = mine.y * f;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  if (lane == 0) sm_red[8 + warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += sm_red[8 + i];
+  // four sets of 64 threads, a thread four channels of every fourth part
+  const int set = tid >> 6, ch = (tid & 63) * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = set; i < parts; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(w.parts + (static_cast<long long>(slot(i)) * kSlotHeads + h) * 256 + ch);
+    const float fi = sm_f[i];
+    o.x = fmaf(fi, v.x, o.x);
+    o.y = fmaf(fi, v.y, o.y);
+    o.z = fmaf(fi, v.z, o.z);
+    o.w = fmaf(fi, v.w, o.w);
+  }
+  if (set > 0) *reinterpret_cast<float4*>(&sm_o[set - 1][ch]) = o;
+  __syncthreads();
+  if (set == 0) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(&sm_o[i][ch]);
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat162 pk[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+    *reinterpret_cast<uint2*>(out + ch) = *reinterpret_cast<const uint2*>(pk);
+  }
+  if (tid == 0) {
+    const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    w.lse[at] = lse;
+    if (c.lse_out != nullptr) c.lse_out[at] = lse;
+  }
+}
+
+// weights[row][i] = decay weights[row][i] + sum_h 2^(x[h][i] - lse[h]), from the scores the decode
+// launch recorded: 4 bytes per position and q head written and read, against the K and V rows' 1024
+// per kv head.  A thread per position, 256 positions at a time.
+__global__ void __launch_bounds__(256) decode_weights_kernel(const akl_decode_t c, const Work w) {
+  __shared__ long long sm_chunks[8];
+  __shared__ float sm_lse[64];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  long long row, before = 0;
+  for (int i = tid; i < b; i += 256) before += (request_of(c, i, row) + kChunk - 1) / kChunk;
+  before = warp_sum(before);
+  if ((tid & 31) == 0) sm_chunks[tid >> 5] = before;
+  const int n = request_of(c, b, row);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid < c.q_heads) sm_lse[tid] = w.lse[static_cast<long long>(b) * c.q_heads + tid];
+  __syncthreads();
+  long long chunk0 = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) chunk0 += sm_chunks[i];
+  for (int i = blockIdx.y * 256 + tid; i < n; i += gridDim.y * 256) {
+    const long long chunk = chunk0 + i / kChunk;
+    if (chunk >= w.max_chunks) {
+      atomicCAS(w.status, 0, AKL_ERR_CAPACITY);
+      break;
+    }
+    const float* x = w.scores + chunk * c.q_heads * kChunk + i % kChunk;
     float total = 0.f;
-    for (int j = 0; slot >= 0 && slot < c.pool_rows && j < c.kv_heads; ++j) {
-      float k[8];
-      unpack8<KV>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + j * 256 + lane * 8), k);
-      for (int h = j * group; h < (j + 1) * group; ++h) {
-        float q[8], x = 0.f;
-        unpack8<AKL_KV_BF16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + b * c.q_stride + h * 256 + lane * 8), q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x = fmaf(q[e] * (c.sm_scale * kLog2e), k[e], x);
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-        total += exp2f(x - lse_ws[b * c.q_heads + h]);
-      }
+#pragma unroll 8
+    for (int h = 0; h < c.q_heads; ++h) {
+      const float v = x[h * kChunk];
+      total += v == -INFINITY ? 0.f : ex2(v - sm_lse[h]);
     }
-    float* w = c.weights + row * c.weights_stride + i;
-    if (lane == 0) *w = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, *w, total);
+    float* dst = c.weights + row * c.weights_stride + i;
+    *dst = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, *dst, total);
   }
 }
 
@@ -174,6 +773,40 @@ int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
   return AKL_OK;
 }
 
+template <int KV, int HB>
+int launch_decode(const akl_decode_t& c, const Work& w, int ctas, cudaStream_t s) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(decode_kernel<KV, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<HB>::kSmem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  if (e == cudaSuccess) {
+    decode_kernel<KV, HB><<<ctas, kThreads, Tile<HB>::kSmem, s>>>(c, w);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) { note_cuda_error(e, "decode_kernel"); return AKL_ERR_CUDA; }
+  return AKL_OK;
+}
+
+// A launch that may be set up while the one before it still runs (it waits for its results itself).
+template <typename... Args>
+int launch_after(void (*kernel)(Args...), dim3 grid, cudaStream_t s, const char* name, Args... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) { note_cuda_error(e, name); return AKL_ERR_CUDA; }
+  return AKL_OK;
+}
+
 }  // namespace
 }  // namespace akl
 
@@ -190,18 +823,30 @@ int akl_paged_decode(const akl_decode_t* c, void* stream) {
   akl_decode_layout_t L;
   int rc = check_decode(c, &L);
   if (rc != AKL_OK) return rc;
+  int sms = 0;
+  if ((rc = device_sm_count(&sms)) != AKL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* lse = reinterpret_cast<float*>(static_cast<uint8_t*>(c->workspace) + L.off_lse);
-  const dim3 grid(c->batch, c->kv_heads), grid_w(c->batch, 64);
-  if (c->kv_dtype == AKL_KV_BF16) decode_kernel<AKL_KV_BF16><<<grid, 256, 0, s>>>(*c, lse);
-  else decode_kernel<AKL_KV_FP16><<<grid, 256, 0, s>>>(*c, lse);
-  if (c->weights != nullptr) {
-    if (c->kv_dtype == AKL_KV_BF16) decode_weights_kernel<AKL_KV_BF16><<<grid_w, 256, 0, s>>>(*c, lse);
-    else decode_weights_kernel<AKL_KV_FP16><<<grid_w, 256, 0, s>>>(*c, lse);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) { note_cuda_error(e, "decode_kernel"); return AKL_ERR_CUDA; }
-  return AKL_OK;
+  uint8_t* ws = static_cast<uint8_t*>(c->workspace);
+  Work w;
+  w.status = reinterpret_cast<int*>(ws + L.off_status);
+  w.info = reinterpret_cast<int4*>(ws + L.off_parts);
+  w.ml = reinterpret_cast<float2*>(ws + L.off_parts + info_bytes(c->plan));
+  w.parts = reinterpret_cast<float*>(ws + L.off_parts + info_bytes(c->plan) + align1k(kMlBytes));
+  w.lse = reinterpret_cast<float*>(ws + L.off_lse);
+  w.scores = c->weights != nullptr ? reinterpret_cast<float*>(ws + L.off_scores) : nullptr;
+  w.max_chunks = (c->plan.max_weight_tokens + kChunk - 1) / kChunk;
+  const int ctas = std::min(sms, kMaxCtas), hb = std::min(c->kv_heads, 4);
+  if (c->kv_dtype == AKL_KV_BF16)
+    rc = hb == 4 ? launch_decode<AKL_KV_BF16, 4>(*c, w, ctas, s)
+                 : (hb == 2 ? launch_decode<AKL_KV_BF16, 2>(*c, w, ctas, s) : launch_decode<AKL_KV_BF16, 1>(*c, w, ctas, s));
+  else
+    rc = hb == 4 ? launch_decode<AKL_KV_FP16, 4>(*c, w, ctas, s)
+                 : (hb == 2 ? launch_decode<AKL_KV_FP16, 2>(*c, w, ctas, s) : launch_decode<AKL_KV_FP16, 1>(*c, w, ctas, s));
+  if (rc != AKL_OK) return rc;
+  rc = launch_after(decode_join_kernel, dim3(c->batch, c->q_heads), s, "decode_join_kernel", *c, w, hb * (c->q_heads / c->kv_heads));
+  if (rc != AKL_OK || c->weights == nullptr) return rc;
+  const int blocks = std::min((c->table_width + 255) / 256, 64);
+  return launch_after(decode_weights_kernel, dim3(c->batch, blocks), s, "decode_weights_kernel", *c, w);
 }
 
 }  // extern "C"

@@ -156,6 +156,23 @@ def test_decode_offsets_beyond_32_bits(pkg, cuda):
                          kv_lens=torch.tensor([n], device=cuda)))
 
 
+def test_decode_reports_weights_beyond_the_plan(pkg, cuda):
+    c = R.case([100, 100], 24, 4, seed=8)
+    ws = pkg.plan_decode_workspace(cuda, max_requests=2, q_heads=24, kv_heads=4, max_weight_tokens=128)
+    weights = torch.zeros(c["page_table"].shape, device=cuda)
+    out, lse = torch.empty_like(c["q"]), torch.empty((2, 24), device=cuda)
+    with pytest.raises(pkg.NativeError) as e:
+        pkg.paged_decode(**c, workspace=ws, out=out, lse_out=lse, weights=weights, return_lse=True, check_status=True)
+    assert e.value.code == -3
+    ref = R.decode(c["q"], c["k_pool"], c["v_pool"], c["page_table"], c["kv_lens"], c["rows"], weights=weights * 0)
+    R.within(out, ref["out"], ref["out_tol"])
+    R.within(lse, ref["lse"], ref["lse_tol"])
+    first = c["rows"][0].long()
+    R.within(weights[first], ref["weights"][first], ref["weights_tol"][first])
+    assert not weights[c["rows"][1].long()].any()
+    pkg.paged_decode(**c, workspace=ws, check_status=True)       # the workspace goes on working
+
+
 def test_decode_in_a_graph_follows_lengths_and_rows(pkg, cuda):
     c = R.case([700, 90, 5], 24, 4, seed=12)
     long = R.case([2000, 1500, 600], 24, 4, seed=13, width=c["page_table"].shape[1] + 1297)
