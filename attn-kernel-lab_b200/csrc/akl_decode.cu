@@ -10,10 +10,11 @@
 //     the device).  A CTA meets a run of requests: those it holds whole it finishes itself, of the
 //     first and the last it may hold a part, whose (m, l, unnormalised out) goes to the workspace for
 //     the join launch.  No atomics: partial states are joined in position order.
-//   * a producer warp gathers the rows by bulk copies, one per position and plane (the kv heads of a
-//     position are neighbours in the pool: 2 KiB at four heads), into a ring of three tiles, with the
-//     page-table entries three tiles ahead.  Rows lie 16 bytes off a multiple of 128 in shared memory,
-//     so that matrix loads meet no bank twice.
+//   * four producer warps gather the rows (the kv heads of a position are neighbours in the pool: 2 KiB
+//     at four heads) into a ring of three tiles with 16-byte asynchronous copies, 512 bytes a warp
+//     instruction, with the page-table entries four tiles ahead.  Rows lie 16 bytes off a multiple of 128 in
+//     shared memory, so that matrix loads meet no bank twice.  (Bulk copies of a row each were measured
+//     first: about 75 cycles of the copy unit apiece, 94 us for 136 MB in rows of 512 bytes.)
 //   * eight warps: four (kv head, 16 positions) tasks times two halves of the output channels.  Both
 //     halves form the scores, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
 //     heads of the kv head on N -- with the heads on M half to three quarters of the tensor work would
@@ -44,8 +45,10 @@ constexpr int kChunk = 64;          // positions per chunk of recorded scores
 constexpr int kMaxGroup = 8;        // query heads per kv head
 constexpr int kMaxCtas = 160;       // CTAs whose partial states the workspace holds (two each)
 constexpr int kStages = 3;
-constexpr int kWarps = 8;           // consumers; one more warp produces
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kWarps = 8;           // consumers
+constexpr int kProducers = 4;       // and the warps that gather for them
+constexpr int kThreads = (kWarps + kProducers) * 32;
+constexpr int kAhead = 4;           // tiles whose page-table entries are on their way
 constexpr int kMinTiles = 1;        // tiles a CTA takes at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr long long kWaitCycles = 4000000000ll;      // ~2 s: a wait that long is a defect
@@ -65,8 +68,9 @@ struct Tile {
   static constexpr int kMerge = kGroups > 1 ? 16384 : 0;
   static constexpr int kOffMerge = kRing;
   static constexpr int kOffMl = kOffMerge + kMerge;  // [8 warps][8 heads] {m, l}
-  static constexpr int kOffMask = kOffMl + 512;      // [kStages] u64: positions of the tile that are there
-  static constexpr int kOffBar = kOffMask + 8 * kStages;
+  static constexpr int kOwn = kPos / kProducers;     // positions of a tile that one producer warp gathers
+  static constexpr int kOffMask = kOffMl + 512;      // [kStages][kProducers] u32: which of them are there
+  static constexpr int kOffBar = kOffMask + 16 * kStages;
   static constexpr int kSmem = kOffBar + 16 * kStages + 16;
 };
 static_assert(Tile<1>::kSmem <= 232448 && Tile<2>::kSmem <= 232448 && Tile<4>::kSmem <= 232448, "shared memory");
@@ -300,84 +304,75 @@ __device__ __forceinline__ void load_q(const akl_decode_t& c, int b, int head0, 
   }
 }
 
-// Producer: the rows of every tile of this CTA's share.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes: 16, or 0 to clear
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// A producer warp: its positions of every tile of this CTA's share.  A row of 512 bytes is one
+// instruction of the warp; rows that are not there are cleared, for 0 * NaN is not 0.
 template <int HB>
 __device__ __forceinline__ void produce(const akl_decode_t& c, uint32_t smem, uint8_t* smem_gen, const Wait& wait,
-                                        Cursor<HB>& at, long long first, int count, int lane) {
+                                        Cursor<HB>& at, long long first, int count, int own, int lane) {
   using T = Tile<HB>;
-  constexpr int kPairs = T::kPos / 16;               // (position, plane) pairs per lane
-  constexpr int kSlots = T::kPos > 32 ? 2 : 1;       // positions per lane
-  long long slot[kStages][kSlots];
-  int block[kStages];
-  // page-table entries of the tile the cursor is at; -1: nothing to read
-  auto look = [&](long long (&s)[kSlots], int& hb) {
+  int slot[kAhead], block[kAhead];
+  // the page-table entry of this lane's position in the tile the cursor is at; -1: nothing to read
+  auto look = [&](int& s, int& hb) {
     hb = at.hb;
-#pragma unroll
-    for (int k = 0; k < kSlots; ++k) {
-      const int i = at.t * T::kPos + (lane + 32 * k) % T::kPos;
-      s[k] = -1;
-      if (i < at.n) {
-        s[k] = load_index(c.page_table, c.idx_dtype, at.row * c.table_stride + i);
-        if (s[k] >= c.pool_rows) s[k] = -1;
-      }
+    s = -1;
+    const int i = at.t * T::kPos + own * T::kOwn + lane;
+    if (lane < T::kOwn && i < at.n) {
+      const long long v = load_index(c.page_table, c.idx_dtype, at.row * c.table_stride + i);
+      if (v >= 0 && v < c.pool_rows) s = static_cast<int>(v);
     }
   };
   at.seek(first);
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) {
+  for (int s = 0; s < kAhead; ++s) {
     if (s < count) {
       if (s > 0) at.next();
       look(slot[s], block[s]);
     }
   }
   const uint32_t bars = smem + T::kOffBar;
-  int issued = 0;
+  const uint32_t dst0 = smem + own * T::kOwn * T::kPitch + lane * 16;
   for (int it = 0; it < count; ++it) {
     const int st = it % kStages;
-    if (it >= kStages && (!wait(bars + (kStages + st) * 8, ((it / kStages) - 1) & 1) || *wait.aborted)) break;
-    long long now[kSlots];
-    int there = 0;
-    unsigned long long mask = 0;
+    const bool free = it < kStages || (wait(bars + (kStages + st) * 8, ((it / kStages) - 1) & 1) && !*wait.aborted);
+    if (!__all_sync(0xffffffffu, free)) break;
+    const int now = slot[0];
+    const unsigned mask = __ballot_sync(0xffffffffu, now >= 0);
+    const long long head0 = static_cast<long long>(block[0]) * (HB * 256) + lane * 8;
+    const uint32_t dst = dst0 + st * T::kStage;
 #pragma unroll
-    for (int k = 0; k < kSlots; ++k) {
-      now[k] = slot[0][k];
-      const unsigned m = __ballot_sync(0xffffffffu, now[k] >= 0) & (T::kPos < 32 ? (1u << (T::kPos & 31)) - 1u : 0xffffffffu);
-      mask |= static_cast<unsigned long long>(m) << (32 * k);
-      there += __popc(m);
-    }
-    const long long head0 = static_cast<long long>(block[0]) * (HB * 256);
-    if (lane == 0) {
-      *reinterpret_cast<volatile unsigned long long*>(smem_gen + T::kOffMask + st * 8) = mask;
-      mbar_expect_tx(bars + st * 8, static_cast<uint32_t>(there) * (2u * T::kRow));
-    }
-    __syncwarp();
+    for (int i = 0; i < T::kOwn; ++i) {
+      const int s = __shfl_sync(0xffffffffu, now, i);
+      const long long row = s < 0 ? 0 : s;
+      const uint32_t bytes = s < 0 ? 0u : 16u;
+      const uint16_t* k = static_cast<const uint16_t*>(c.k_pool) + row * c.k_stride + head0;
+      const uint16_t* v = static_cast<const uint16_t*>(c.v_pool) + row * c.v_stride + head0;
 #pragma unroll
-    for (int p = 0; p < kPairs; ++p) {
-      const int pair = lane + 32 * p, pos = pair % T::kPos, plane = pair / T::kPos;
-      const long long s = now[kSlots == 2 ? p & 1 : 0];
-      if (s >= 0) {
-        const uint16_t* src = plane == 0 ? static_cast<const uint16_t*>(c.k_pool) + s * c.k_stride + head0
-                                         : static_cast<const uint16_t*>(c.v_pool) + s * c.v_stride + head0;
-        bulk_g2s(smem + st * T::kStage + plane * T::kPlane + pos * T::kPitch, src, T::kRow, bars + st * 8);
+      for (int e = 0; e < HB; ++e) {
+        copy16(dst + i * T::kPitch + e * 512, k + e * 256, bytes);
+        copy16(dst + T::kPlane + i * T::kPitch + e * 512, v + e * 256, bytes);
       }
     }
+    // one arrival per thread once its copies landed, and one that publishes the mask
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bars + st * 8) : "memory");
+    if (lane == 0) {
+      reinterpret_cast<volatile uint32_t*>(smem_gen + T::kOffMask + st * 16)[own] = mask;
+      mbar_arrive(bars + st * 8);
+    }
 #pragma unroll
-    for (int s = 0; s + 1 < kStages; ++s) {
+    for (int s = 0; s + 1 < kAhead; ++s) {
       block[s] = block[s + 1];
-#pragma unroll
-      for (int k = 0; k < kSlots; ++k) slot[s][k] = slot[s + 1][k];
+      slot[s] = slot[s + 1];
     }
-    if (it + kStages < count) {
+    if (it + kAhead < count) {
       at.next();
-      look(slot[kStages - 1], block[kStages - 1]);
+      look(slot[kAhead - 1], block[kAhead - 1]);
     }
-    issued = it + 1;
   }
-  // no copy may outlive the CTA: they land (or the limit passes) before this warp ends
-  for (int it = issued > kStages ? issued - kStages : 0; it < issued; ++it) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bars + (it % kStages) * 8, (it / kStages) & 1) && clock64() - t0 < kWaitCycles) {}
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");       // no copy outlives its thread
 }
 
 template <int KV, int HB>
@@ -391,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   if (threadIdx.x == 0) {
     sm_aborted = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem + T::kOffBar + i * 8, 1);
+      mbar_init(smem + T::kOffBar + i * 8, kProducers * 33);
       mbar_init(smem + T::kOffBar + (kStages + i) * 8, kWarps);
     }
     mbar_init_fence();
@@ -406,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   __syncthreads();
   const Wait wait{w.status, &sm_aborted};
 
-  if (warp == kWarps) {
-    produce<HB>(c, smem, smem_gen, wait, at, first, count, lane);
+  if (warp >= kWarps) {
+    produce<HB>(c, smem, smem_gen, wait, at, first, count, warp - kWarps, lane);
     return;
   }
 
@@ -436,9 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
     }
     const int st = it % kStages;
     const uint32_t stage = smem + st * T::kStage;
-    if (ok) ok = wait(bars + st * 8, (it / kStages) & 1);
+    if (ok) ok = __all_sync(0xffffffffu, wait(bars + st * 8, (it / kStages) & 1));
     if (ok) {
-      const unsigned there = static_cast<unsigned>(*reinterpret_cast<volatile unsigned long long*>(smem_gen + T::kOffMask + st * 8) >> (16 * tg)) & 0xFFFFu;
+      unsigned there = 0;               // positions of this warp's sixteen that are there
+#pragma unroll
+      for (int i = 0; i < 16 / T::kOwn; ++i)
+        there |= reinterpret_cast<volatile uint32_t*>(smem_gen + T::kOffMask + st * 16)[tg * (16 / T::kOwn) + i] << (i * T::kOwn);
       // scores of 16 positions x 8 heads: thread has positions g, g + 8 of heads 2 quad, 2 quad + 1.
       // Four chains of four products keep the sums short, in time and in rounding.
       float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -457,14 +455,6 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
         if (there != 0xFFFFu) {
           if (!((there >> g) & 1u)) x[0] = x[1] = -INFINITY;
           if (!((there >> (g + 8)) & 1u)) x[2] = x[3] = -INFINITY;
-          // V rows that were not read hold anything: clear them (this warp's channels), for 0 * NaN is not 0.
-          // The next copy into them follows this warp's arrival, behind the proxy fence.
-          for (unsigned gone = ~there & 0xFFFFu; gone != 0u; gone &= gone - 1u) {
-            const uint32_t at_row = stage + T::kPlane + (tg * 16 + __ffs(gone) - 1) * T::kPitch + unit * 512 + half * 256;
-            if (lane < 16) st_shared_v4(at_row + lane * 16, 0u, 0u, 0u, 0u);
-          }
-          fence_async_smem();
-          __syncwarp();
         }
       }
       if (w.scores != nullptr && half == 0) {
@@ -756,6 +746,7 @@ int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
   if (!(c->sm_scale > 0.f) || !(c->weight_decay >= 0.f && c->weight_decay <= 1.f)) return AKL_ERR_INVALID;
   if (c->rows == nullptr && c->table_rows < c->batch) return AKL_ERR_INVALID;
   if (c->q_heads % c->kv_heads || c->q_heads / c->kv_heads > kMaxGroup) return AKL_ERR_UNSUPPORTED;
+  if (c->pool_rows >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;      // slots travel in 32 bits
   if (c->kv_heads != 1 && c->kv_heads != 2 && c->kv_heads != 4 && c->kv_heads != 8) return AKL_ERR_UNSUPPORTED;
   if (c->k_stride < c->kv_heads * 256 || c->v_stride < c->kv_heads * 256 || c->q_stride < c->q_heads * 256 ||
       c->table_stride < c->table_width)

@@ -195,8 +195,9 @@ def check_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
     if batch < 1:
         _reject("q must hold at least one request: an empty batch must be skipped by the caller", field="q",
                 value=batch, supported=">= 1")
-    if k_pool.shape[0] < 1:
-        _reject("k_pool must hold at least one slot", field="k_pool", value=tuple(k_pool.shape), supported=">= 1")
+    if not 1 <= k_pool.shape[0] < 1 << 31:
+        _reject(f"k_pool must hold 1 to 2^31 - 1 slots, got {k_pool.shape[0]}", field="k_pool",
+                value=tuple(k_pool.shape), supported="1 .. 2^31 - 1")
     _check_rows("q", q, q_heads)
     _check_rows("k_pool", k_pool, kv_heads)
     _check_rows("v_pool", v_pool, kv_heads)
