@@ -620,23 +620,29 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   }
 }
 
-// Join of the partial states of one (request, q head): lse = log2 sum_i l_i 2^m_i, out = sum_i 2^(m_i - lse) O_i,
-// in position order.  A request without positions gets its zeros here.
-__global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, const Work w, int hb_heads) {
-  __shared__ float sm_f[kMaxCtas + 1];
+// Join of the partial states of a (request, q head): lse = log2 sum_i l_i 2^m_i, out = sum_i 2^(m_i - lse) O_i,
+// in position order.  A request without positions gets its zeros here; one that a single CTA held
+// has its result already.  Latency bound (a request's parts are read from L2 once): what counts is how
+// many of the loads are in flight together.
+
+// Few requests, so up to all 148 parts of one: a CTA takes 64 channels, sixteen sets of sixteen threads
+// every sixteenth part, all of whose loads are issued before the factors that they wait for.
+__global__ void __launch_bounds__(256) decode_join_wide_kernel(const akl_decode_t c, const Work w, int hb_heads) {
+  constexpr int kSets = 16, kEach = kMaxCtas / kSets;
+  __shared__ float sm_f[kMaxCtas];
   __shared__ float sm_red[16];
-  __shared__ __align__(16) float sm_o[3][256];   // read and written as float4
-  const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ __align__(16) float sm_o[kSets][64];       // read and written as float4
+  const int b = blockIdx.x, head = blockIdx.y, ch0 = blockIdx.z * 64, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long long row;
   const int n = request_of(c, b, row);
   const int hb = head / hb_heads, h = head - hb * hb_heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + (static_cast<long long>(b) * c.q_heads + head) * 256;
   const long long at = static_cast<long long>(b) * c.q_heads + head;
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + at * 256 + ch0;
   if (n == 0) {
-    out[tid] = __float2bfloat16_rn(0.f);
-    if (tid == 0) {
+    if (tid < 64) out[tid] = __float2bfloat16_rn(0.f);
+    if (tid == 0 && ch0 == 0) {
       w.lse[at] = -INFINITY;
       if (c.lse_out != nullptr) c.lse_out[at] = -INFINITY;
     }
@@ -644,10 +650,15 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, 
   }
   const int4 info = w.info[b * 2 + hb];
   const int parts = info.z - info.y + 1;
-  if (parts == 1) return;                            // one CTA held the request and wrote the result
-  auto slot = [&](int i) { return i == 0 ? info.x : 2 * (info.y + i); };
+  if (parts == 1) return;
+  auto slot = [&](int i) { return (i == 0 ? info.x : 2 * (info.y + i)) * kSlotHeads + h; };
+  const int set = tid >> 4, ch = (tid & 15) * 4;
+  float4 v[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (set + k * kSets < parts) v[k] = *reinterpret_cast<const float4*>(w.parts + static_cast<long long>(slot(set + k * kSets)) * 256 + ch0 + ch);
   float2 mine = make_float2(-INFINITY, 0.f);
-  if (tid < parts) mine = w.ml[slot(tid) * kSlotHeads + h];
+  if (tid < parts) mine = w.ml[slot(tid)];
   float top = warp_max(mine.x);
   if (lane == 0) sm_red[warp] = top;
   __syncthreads();
@@ -665,35 +676,77 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, 
   sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += sm_red[8 + i];
-  // four sets of 64 threads, a thread four channels of every fourth part
-  const int set = tid >> 6, ch = (tid & 63) * 4;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = set; i < parts; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(w.parts + (static_cast<long long>(slot(i)) * kSlotHeads + h) * 256 + ch);
-    const float fi = sm_f[i];
-    o.x = fmaf(fi, v.x, o.x);
-    o.y = fmaf(fi, v.y, o.y);
-    o.z = fmaf(fi, v.z, o.z);
-    o.w = fmaf(fi, v.w, o.w);
-  }
-  if (set > 0) *reinterpret_cast<float4*>(&sm_o[set - 1][ch]) = o;
-  __syncthreads();
-  if (set == 0) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(&sm_o[i][ch]);
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
+  for (int k = 0; k < kEach; ++k)
+    if (set + k * kSets < parts) {
+      const float fi = sm_f[set + k * kSets];
+      o.x = fmaf(fi, v[k].x, o.x);
+      o.y = fmaf(fi, v[k].y, o.y);
+      o.z = fmaf(fi, v[k].z, o.z);
+      o.w = fmaf(fi, v[k].w, o.w);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    __nv_bfloat162 pk[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
-    *reinterpret_cast<uint2*>(out + ch) = *reinterpret_cast<const uint2*>(pk);
+  *reinterpret_cast<float4*>(&sm_o[set][ch]) = o;
+  __syncthreads();
+  if (tid < 64) {
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) total += sm_o[i][tid];
+    out[tid] = __float2bfloat16_rn(sum == 0.f ? 0.f : total / sum);
   }
-  if (tid == 0) {
+  if (tid == 0 && ch0 == 0) {
     const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    w.lse[at] = lse;
+    if (c.lse_out != nullptr) c.lse_out[at] = lse;
+  }
+}
+
+// Many requests, so few parts of each: a warp per (request, q head), a lane eight channels, one part
+// after the other with a running maximum.
+__global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, const Work w, int hb_heads) {
+  const int lane = threadIdx.x & 31;
+  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const bool in = at < static_cast<long long>(c.batch) * c.q_heads;
+  const int b = in ? static_cast<int>(at / c.q_heads) : 0, head = in ? static_cast<int>(at - static_cast<long long>(b) * c.q_heads) : 0;
+  const int hb = head / hb_heads, h = head - hb * hb_heads;
+  long long row;
+  const int n = request_of(c, b, row);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!in) return;
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + at * 256 + lane * 8;
+  float m = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = 0.f;
+  if (n > 0) {
+    const int4 info = w.info[b * 2 + hb];
+    const int parts = info.z - info.y + 1;
+    if (parts == 1) return;
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i) {
+      const int s = (i == 0 ? info.x : 2 * (info.y + i)) * kSlotHeads + h;
+      const float2 ml = w.ml[s];
+      const float4* src = reinterpret_cast<const float4*>(w.parts + static_cast<long long>(s) * 256 + lane * 8);
+      const float4 v0 = src[0], v1 = src[1];
+      const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+      const float top = fmaxf(m, ml.x), safe = top == -INFINITY ? 0.f : top;
+      const float keep = ex2(m - safe), add = ex2(ml.x - safe);
+      m = top;
+      l = l * keep + ml.y * add;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = o[e] * keep + v[e] * add;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t pk[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+    pk[e] = *reinterpret_cast<const uint32_t*>(&t);
+  }
+  *reinterpret_cast<uint4*>(out) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+  if (lane == 0) {
+    const float lse = l == 0.f ? -INFINITY : m + log2f(l);
     w.lse[at] = lse;
     if (c.lse_out != nullptr) c.lse_out[at] = lse;
   }
@@ -834,7 +887,11 @@ int akl_paged_decode(const akl_decode_t* c, void* stream) {
     rc = hb == 4 ? launch_decode<AKL_KV_FP16, 4>(*c, w, ctas, s)
                  : (hb == 2 ? launch_decode<AKL_KV_FP16, 2>(*c, w, ctas, s) : launch_decode<AKL_KV_FP16, 1>(*c, w, ctas, s));
   if (rc != AKL_OK) return rc;
-  rc = launch_after(decode_join_kernel, dim3(c->batch, c->q_heads), s, "decode_join_kernel", *c, w, hb * (c->q_heads / c->kv_heads));
+  // the wide join while its CTAs fit the GPU in about two waves; past that a request has few parts
+  const int64_t pairs = static_cast<int64_t>(c->batch) * c->q_heads;
+  const int hb_heads = hb * (c->q_heads / c->kv_heads);
+  rc = pairs * 4 <= 8 * sms ? launch_after(decode_join_wide_kernel, dim3(c->batch, c->q_heads, 4), s, "decode_join_wide_kernel", *c, w, hb_heads)
+                            : launch_after(decode_join_kernel, dim3(static_cast<unsigned>((pairs + 7) / 8)), s, "decode_join_kernel", *c, w, hb_heads);
   if (rc != AKL_OK || c->weights == nullptr) return rc;
   const int blocks = std::min((c->table_width + 255) / 256, 64);
   return launch_after(decode_weights_kernel, dim3(c->batch, blocks), s, "decode_weights_kernel", *c, w);
