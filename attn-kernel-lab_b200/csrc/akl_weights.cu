@@ -1,5 +1,28 @@
 // Attention weights of an extend: weights[i] (+)= sum over rows t and q heads h with i <= prefix + t of
 // 2^(c <q[t][h], k_i> - lse[t][h]), c = sm_scale log2 e.
+//
+// One product of 256 multiply-adds and one exponential per (position, row, head), and a sum over rows and
+// heads: tensor pipe (4096 multiply-adds a cycle and SM) and exponential unit (16 a cycle and SM) need
+// the same time, everything else is small.  The product is formed transposed, D = K Q^T, so that
+//
+//   * a TMEM lane is a position and the sum over rows and heads runs along the columns: every thread
+//     adds up numbers of its own, nothing is exchanged, and the scores are never written;
+//   * K is the A operand and stays in TMEM (256 positions, 256 columns) while the packed (row, head) pairs
+//     of the kv head stream through shared memory as B, 128 at a time.  With K in shared memory an
+//     M128 N128 K16 product reads 8 KiB in its 64 cycles, all that shared memory gives.
+//
+// The rows are packed once per call into swizzled images of 128 rows (row = t group + head, so short
+// windows fill their tiles), with the factor and the LSE of each; a tile is then one bulk copy.
+// A unit is (256 positions, kv head, 128 rows).  The units, position tile by position tile and head by
+// head, are one sequence of which every CTA takes an equal share; tiles above the diagonal are not
+// in it.  A CTA's first piece may continue the one of the CTA before it and then goes to a place of its own; the last launch
+// adds the pieces of a position in a fixed order.
+//
+// Rounding: scores and sums are 32-bit.  BF16 queries meet a BF16 pool unchanged; for an FP16 pool
+// a row is divided by the power of two of its largest element and rounded to FP16: exact down to
+// 2^-17 of that element, 2^-25 of it below.
+#include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "akl_common.cuh"
@@ -9,46 +32,432 @@ namespace akl {
 
 namespace {
 
+using namespace ptx;
+
 constexpr int kMaxGroup = 8;
+constexpr int kMaxCtas = 160;
+constexpr int kRows = 128;                          // packed rows of a tile
+constexpr int kPos = 256;                           // positions of a unit: two TMEM lane sets
+constexpr int kImage = 4 * kPlaneBytes;             // four planes of 64 channels, 128-byte swizzle
+constexpr int kTileBytes = kImage + 2 * kRows * 4;  // and per row {factor}[128], {-lse}[128]
+constexpr int kStages = 3;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 3) * 32;      // + two warps that issue products, one that fetches rows
+constexpr uint32_t kTmemCols = 512, kColD = 0, kColK = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr long long kWaitCycles = 4000000000ll;     // ~2 s: a wait that long is a defect
+
+inline uint64_t align1k(uint64_t x) { return (x + 1023) / 1024 * 1024; }
 
 int weights_layout(const akl_weights_plan_t& p, akl_weights_layout_t* o) {
   if (p.max_kv_len < 1 || p.max_q_len < 1 || p.q_heads < 1 || p.kv_heads < 1) return AKL_ERR_INVALID;
   if (p.q_heads % p.kv_heads || p.q_heads / p.kv_heads > kMaxGroup) return AKL_ERR_UNSUPPORTED;
+  if (p.max_q_len >= (1 << 27) || p.max_kv_len >= (1 << 30)) return AKL_ERR_UNSUPPORTED;    // 32-bit packed rows and positions
   std::memset(o, 0, sizeof(*o));
-  o->total_bytes = 1024;
+  const uint64_t tiles = (static_cast<uint64_t>(p.max_q_len) * (p.q_heads / p.kv_heads) + kRows - 1) / kRows;
+  const uint64_t pos = (static_cast<uint64_t>(p.max_kv_len) + kPos - 1) / kPos * kPos;
+  uint64_t off = 1024;
+  o->off_q = off;
+  off += align1k(tiles * p.kv_heads * kTileBytes);
+  o->off_parts = off;
+  off += align1k(pos * p.kv_heads * 4) + align1k(static_cast<uint64_t>(kMaxCtas) * kPos * 4);
+  o->total_bytes = off;
   return AKL_OK;
 }
 
-// One warp per position, a lane eight channels.
-template <int KV>
-__global__ void __launch_bounds__(256) extend_weights_kernel(akl_weights_t c) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
-  const int i = blockIdx.x * 8 + warp;
-  if (i >= c.N) return;
-  const long long slot = load_index(c.idx, c.idx_dtype, i);
-  float total = 0.f;
-  for (int j = 0; slot >= 0 && slot < c.pool_rows && j < c.kv_heads; ++j) {
-    float k[8];
-    unpack8<KV>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + j * 256 + lane * 8), k);
-    float head = 0.f;
-    for (int t = max(0, i - c.prefix); t < c.T; ++t) {
-      float part = 0.f;
-      for (int h = j * group; h < (j + 1) * group; ++h) {
-        float q[8], x = 0.f;
-        unpack8<AKL_KV_BF16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + t * c.q_stride + h * 256 + lane * 8), q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x = fmaf(q[e], k[e], x);
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-        const float lse = c.lse[static_cast<long long>(t) * c.q_heads + h];
-        if (!isinf(lse)) part += exp2f(fmaf(x, c.sm_scale * kLog2e, -lse));
-      }
-      head += part;
-    }
-    total += head;
+// The sequence of units, from the call alone.
+struct Units {
+  int group, heads, tiles, ptiles, full, prefix;    // full: position tiles that every row tile sees
+  long long total;
+  long long ctas;
+  __host__ __device__ int first_tile(int p) const { // row tiles before this one see nothing of position tile p
+    const long long n0 = static_cast<long long>(p) * kPos - prefix;
+    return n0 <= 0 ? 0 : static_cast<int>(n0 * group / kRows);
   }
-  if (lane == 0) c.weights[i] = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, c.weights[i], total);
+  __host__ __device__ int count(int p) const {
+    const int f = first_tile(p);
+    return f < tiles ? tiles - f : 0;
+  }
+  __host__ __device__ long long start(int p) const {
+    long long u = static_cast<long long>(p < full ? p : full) * tiles;
+    for (int i = full; i < p; ++i) u += count(i);
+    return u * heads;
+  }
+};
+
+struct Work {
+  const uint8_t* images;     // [kv head][tile][kTileBytes]
+  float* sums;               // [kv head][position]: pieces that begin a (position tile, kv head)
+  float* more;               // [CTA][kPos]: first pieces that continue one
+  int* status;
+  int pos_cap;               // positions between two kv heads of sums
+};
+
+// One warp per packed row: its image row in the pool's type, factor and -lse.
+template <int KV>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const akl_weights_t c, uint8_t* images, int tiles) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int group = c.q_heads / c.kv_heads, j = blockIdx.y, lane = threadIdx.x & 31;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), tile = r / kRows, row = r % kRows;
+  uint8_t* image = images + (static_cast<long long>(j) * tiles + tile) * kTileBytes;
+  const int t = r / group, h = j * group + r - t * group;
+  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+  float factor = 0.f, neg = -INFINITY;
+  if (t < c.T) {
+    raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + t * c.q_stride + h * 256 + lane * 8);
+    factor = c.sm_scale * kLog2e;
+    const float lse = __ldg(c.lse + static_cast<long long>(t) * c.q_heads + h);
+    neg = isinf(lse) ? -INFINITY : -lse;             // a row that saw no key adds nothing
+    if (KV == AKL_KV_FP16) {
+      float x[8], top = 0.f;
+      unpack8<AKL_KV_BF16>(raw, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+      top = warp_max(top);
+      // 2^e <= top < 2^(e+1), with both 2^e and 2^-e normal; 1 for a row of zeros or of infinities
+      int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xFFu) - 127;
+      e = (top == 0.f || e == 128) ? 0 : max(-126, min(126, e));
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      uint32_t pk[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 v = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
+        pk[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      raw = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+    }
+  }
+  *reinterpret_cast<uint4*>(image + (lane >> 3) * kPlaneBytes + swz128(row, (lane & 7) * 16)) = raw;
+  if (lane == 0) {
+    float* f = reinterpret_cast<float*>(image + kImage);
+    f[row] = factor;
+    f[kRows + row] = neg;
+  }
+}
+
+struct Bars {
+  uint32_t base;
+  __device__ uint32_t q_full(int s) const { return base + s * 8; }
+  __device__ uint32_t q_empty(int s) const { return base + (kStages + s) * 8; }
+  __device__ uint32_t d_full(int s) const { return base + (2 * kStages + s) * 8; }
+  __device__ uint32_t d_empty(int s) const { return base + (2 * kStages + 2 + s) * 8; }
+  __device__ uint32_t k_full() const { return base + (2 * kStages + 4) * 8; }
+};
+constexpr int kBars = 2 * kStages + 5;
+constexpr int kOffRed = kStages * kTileBytes;       // [2][kPos] floats, behind the row tiles
+constexpr int kOffBar = kOffRed + 2 * kPos * 4;
+constexpr int kOffMisc = kOffBar + kBars * 8 + 8;
+constexpr int kSmem = kOffMisc + 64 + 1024;         // + alignment slack
+static_assert(kSmem <= 232448 && kTileBytes % 1024 == 0, "shared memory");
+
+struct Wait {
+  int* status;
+  volatile int* aborted;     // shared memory
+  // Every waiter observes every phase of its barriers in order.  False after ~2 s, or once another
+  // thread of the CTA gave up; the status word then says so.
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    long long t0 = 0;
+    for (uint32_t spin = 1;; ++spin) {
+      if (mbar_try_wait(bar, parity)) return true;
+      if ((spin & 0x3FFu) == 0) {
+        if (t0 == 0) t0 = clock64();
+        if (*aborted || clock64() - t0 > kWaitCycles) {
+          *aborted = 1;
+          atomicCAS(status, 0, AKL_ERR_TIMEOUT);
+          return false;
+        }
+      }
+    }
+  }
+};
+
+// Instruction descriptor of kind::f16: both operands K-major and of one type (f16 or bf16), fp32 D.
+template <int KV>
+__host__ __device__ constexpr uint32_t idesc_16(int m, int n) {
+  return (1u << 4) | ((KV == AKL_KV_BF16 ? 1u : 0u) << 7) | ((KV == AKL_KV_BF16 ? 1u : 0u) << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T; one thread issues.
+__device__ __forceinline__ void mma_16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+
+// What this CTA's share holds next: position tile p, kv head j, row tiles [r, r_end).
+struct Piece {
+  int p, j, r, r_end;
+  bool begins;
+};
+__device__ __forceinline__ Piece first_piece(const Units& u, long long at, long long count) {
+  Piece x;
+  const long long per = static_cast<long long>(u.heads) * u.tiles;
+  long long in;
+  if (at < per * u.full) {
+    x.p = static_cast<int>(at / per);
+    in = at - per * x.p;
+  } else {
+    in = at - per * u.full;
+    for (x.p = u.full;; ++x.p) {
+      const long long n = static_cast<long long>(u.heads) * u.count(x.p);
+      if (in < n || x.p + 1 >= u.ptiles) break;
+      in -= n;
+    }
+  }
+  const int n = max(1, u.count(x.p));
+  x.j = static_cast<int>(in / n);
+  const int skip = static_cast<int>(in - static_cast<long long>(x.j) * n);
+  x.begins = skip == 0;
+  x.r = u.first_tile(x.p) + skip;
+  x.r_end = static_cast<int>(min(static_cast<long long>(u.tiles), x.r + count));
+  return x;
+}
+// The piece behind x; `left` units of the share remain, at least one.
+__device__ __forceinline__ Piece next_piece(const Units& u, Piece x, long long left) {
+  if (++x.j == u.heads) { x.j = 0; ++x.p; }
+  x.begins = true;
+  x.r = u.first_tile(x.p);
+  x.r_end = static_cast<int>(min(static_cast<long long>(u.tiles), x.r + left));
+  return x;
+}
+
+// 2^(s factor - lse) of 32 columns, added up; columns outside [low, high) count nothing.
+template <int KV, bool kMask>
+__device__ __forceinline__ float add_columns(const uint32_t (&v)[32], const float* rows, float factor, int low, int high) {
+  f2 acc[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(rows + kRows + i);
+    float4 f = make_float4(factor, factor, factor, factor);
+    if (KV == AKL_KV_FP16) f = *reinterpret_cast<const float4*>(rows + i);
+    float p[4];
+    unpack2(fma2p(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), pack2(f.x, f.y), pack2(l.x, l.y)), p[0], p[1]);
+    unpack2(fma2p(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), pack2(f.z, f.w), pack2(l.z, l.w)), p[2], p[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      p[e] = ex2(p[e]);
+      if (kMask && !(i + e >= low && i + e < high)) p[e] = 0.f;
+    }
+    acc[0] = add2p(acc[0], pack2(p[0], p[1]));
+    acc[1] = add2p(acc[1], pack2(p[2], p[3]));
+  }
+  float a, b;
+  unpack2(add2p(acc[0], acc[1]), a, b);
+  return a + b;
+}
+
+template <int KV>
+__global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_weights_t c, const Units u, const Work w) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem_gen = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem = smem_u32(smem_gen);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Bars bars{smem + kOffBar};
+  volatile int* aborted = reinterpret_cast<volatile int*>(smem_gen + kOffMisc);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + kOffMisc + 16);
+  const Wait wait{w.status, aborted};
+  if (threadIdx.x == 0) {
+    *aborted = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bars.q_full(s), 1);
+      mbar_init(bars.q_empty(s), kEpiWarps + 2);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bars.d_full(s), 1);
+      mbar_init(bars.d_empty(s), kEpiWarps);
+    }
+    mbar_init(bars.k_full(), kEpiWarps);
+    mbar_init_fence();
+  }
+  if (warp == kEpiWarps) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const long long first = u.total * blockIdx.x / u.ctas;
+  const int count = static_cast<int>(u.total * (blockIdx.x + 1) / u.ctas - first);
+  const Piece begin = first_piece(u, first, count);
+
+  if (warp >= kEpiWarps) {
+    if (lane == 0) {
+      Piece x = begin;
+      if (warp == kEpiWarps + 2) {
+        // ---- row tiles, one bulk copy each
+        asm volatile("griddepcontrol.wait;" ::: "memory");        // they are packed by the launch before
+        int issued = 0;
+        for (int it = 0; it < count; ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && (!wait(bars.q_empty(s), (it / kStages - 1) & 1) || *aborted)) break;
+          mbar_expect_tx(bars.q_full(s), kTileBytes);
+          bulk_g2s(smem + s * kTileBytes, w.images + (static_cast<long long>(x.j) * u.tiles + x.r) * kTileBytes, kTileBytes, bars.q_full(s));
+          issued = it + 1;
+          if (++x.r == x.r_end && issued < count) x = next_piece(u, x, count - issued);
+        }
+        // no copy may outlive the CTA: they land (or the limit passes) before this thread ends
+        for (int it = issued > kStages ? issued - kStages : 0; it < issued; ++it) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(bars.q_full(it % kStages), (it / kStages) & 1) && clock64() - t0 < kWaitCycles) {}
+        }
+      } else {
+        // ---- products of one set of 128 positions: 16 of K = 16 per row tile.  Two threads issue, for an
+        // issue takes its thread longer than the product takes the tensor pipe.
+        const int sub = warp - kEpiWarps;
+        const uint32_t d = tmem + kColD + sub * 128, a = tmem + kColK + sub * 128;
+        int piece = 0;
+        bool fresh = true;
+        for (int it = 0; it < count; ++it) {
+          const int s = it % kStages;
+          if (fresh && !wait(bars.k_full(), piece & 1)) break;
+          if (!wait(bars.q_full(s), (it / kStages) & 1)) break;
+          if (it > 0 && !wait(bars.d_empty(sub), (it - 1) & 1)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            mma_16_ts(d, a + k * 8, smem_desc_k128(smem + s * kTileBytes + (k >> 2) * kPlaneBytes + (k & 3) * 32),
+                      idesc_16<KV>(128, kRows), k > 0 ? 1u : 0u);
+          tc_commit(bars.d_full(sub));
+          tc_commit(bars.q_empty(s));
+          fresh = ++x.r == x.r_end;
+          if (fresh && it + 1 < count) {
+            x = next_piece(u, x, count - it - 1);
+            ++piece;
+          }
+        }
+      }
+    }
+  } else {
+    // ---- positions: lane set `warp & 3` of both halves of the tile, columns 64 (warp / 4) ..
+    const int quarter = warp & 3, side = warp >> 2;
+    const int at = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const float factor = c.sm_scale * kLog2e;
+    float* red = reinterpret_cast<float*>(smem_gen + kOffRed);
+    Piece x = begin;
+    int it = 0, piece = 0;
+    bool ok = true;
+    while (it < count) {
+      // K of position 128 side + at into TMEM.  Every product of the piece before has been waited for.
+      {
+        const long long n = static_cast<long long>(x.p) * kPos + side * 128 + at;
+        const uint4* src = nullptr;
+        if (n < c.N) {
+          const long long slot = load_index(c.idx, c.idx_dtype, n);
+          if (slot >= 0 && slot < c.pool_rows)
+            src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + x.j * 256);
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int part = 0; part < 4; part += 2) {
+          uint32_t v[2][32];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint4 raw = src != nullptr ? __ldg(src + (part + b) * 8 + i) : make_uint4(0u, 0u, 0u, 0u);
+              v[b][4 * i] = raw.x;
+              v[b][4 * i + 1] = raw.y;
+              v[b][4 * i + 2] = raw.z;
+              v[b][4 * i + 3] = raw.w;
+            }
+          tmem_st32(lanes + kColK + side * 128 + part * 32, v[0]);
+          tmem_st32(lanes + kColK + side * 128 + part * 32 + 32, v[1]);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.k_full());
+      }
+      float sum[2] = {0.f, 0.f};
+      const long long n0 = static_cast<long long>(x.p) * kPos - c.prefix;     // first position, against row 0's diagonal
+      for (; x.r < x.r_end; ++x.r, ++it) {
+        const int s = it % kStages;
+        if (ok) ok = wait(bars.q_full(s), (it / kStages) & 1);
+        const float* rows = reinterpret_cast<const float*>(smem_gen + s * kTileBytes + kImage) + side * 64;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          if (ok) ok = wait(bars.d_full(sub), it & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) continue;
+          tc_fence_after();
+          uint32_t v[2][32];
+          tmem_ld32(lanes + kColD + sub * 128 + side * 64, v[0]);
+          tmem_ld32(lanes + kColD + sub * 128 + side * 64 + 32, v[1]);
+          tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.d_empty(sub));
+          // packed rows from (n - prefix) group on see position n; the last tile may be short
+          const int tile0 = x.r * kRows + side * 64;
+          const int short_by = u.tiles * kRows - c.T * u.group;
+          const bool cut = (n0 + sub * 128 + 127) * u.group > x.r * kRows || (x.r + 1 == u.tiles && short_by > 0);
+          if (!cut) {
+            sum[sub] += add_columns<KV, false>(v[0], rows, factor, 0, 32) + add_columns<KV, false>(v[1], rows + 32, factor, 0, 32);
+          } else {
+            const long long low = (n0 + sub * 128 + at) * u.group - tile0;
+            const int lo = static_cast<int>(max(-64ll, min(64ll, low)));
+            const int hi = min(64, c.T * u.group - tile0);
+            sum[sub] += add_columns<KV, true>(v[0], rows, factor, lo, hi) + add_columns<KV, true>(v[1], rows + 32, factor, lo - 32, hi - 32);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.q_empty(s));
+      }
+      // the two halves of the columns meet; a piece's buffer is used again two pieces, so one barrier, later
+      if (!ok) sum[0] = sum[1] = __int_as_float(0x7FC00000);
+      float* meet = red + (piece & 1) * kPos;
+      if (side == 1) {
+        meet[at] = sum[0];
+        meet[128 + at] = sum[1];
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (side == 0) {
+        float* dst = x.begins ? w.sums + static_cast<long long>(x.j) * w.pos_cap + static_cast<long long>(x.p) * kPos
+                              : w.more + static_cast<long long>(blockIdx.x) * kPos;
+        dst[at] = sum[0] + meet[at];
+        dst[128 + at] = sum[1] + meet[128 + at];
+      }
+      ++piece;
+      if (it < count) x = next_piece(u, x, count - it);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kEpiWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// One CTA per position tile: heads in order, of each the piece that begins it and those that go on.
+__global__ void __launch_bounds__(kPos) add_pieces_kernel(const akl_weights_t c, const Units u, const Work w) {
+  const int p = blockIdx.x;
+  const long long n = static_cast<long long>(p) * kPos + threadIdx.x;
+  const int units = u.count(p);
+  const long long base = u.start(p);
+  bool there = false;
+  if (n < c.N) {
+    const long long slot = load_index(c.idx, c.idx_dtype, n);
+    there = slot >= 0 && slot < c.pool_rows;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (n >= c.N) return;
+  float total = 0.f;
+  for (int j = 0; units > 0 && there && j < u.heads; ++j) {
+    const long long at = base + static_cast<long long>(j) * units;
+    float v = w.sums[static_cast<long long>(j) * w.pos_cap + n];
+    // CTAs whose share begins inside (at, at + units)
+    const long long lo = ((at + 1) * u.ctas + u.total - 1) / u.total;
+    const long long hi = min(u.ctas, ((at + units) * u.ctas + u.total - 1) / u.total);
+    for (long long i = lo; i < hi; ++i) v += w.more[i * kPos + threadIdx.x];
+    total += v;
+  }
+  c.weights[n] = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, c.weights[n], total);
 }
 
 int check_weights(const akl_weights_t* c, akl_weights_layout_t* L) {
@@ -74,6 +483,39 @@ int check_weights(const akl_weights_t* c, akl_weights_layout_t* L) {
   return AKL_OK;
 }
 
+template <int KV>
+int launch_weights(const akl_weights_t& c, const Units& u, const Work& w, uint8_t* images, cudaStream_t s) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(extend_weights_kernel<KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  if (e == cudaSuccess) {
+    pack_rows_kernel<KV><<<dim3(u.tiles * (kRows / 8), c.kv_heads), 256, 0, s>>>(c, images, u.tiles);
+    e = cudaGetLastError();
+  }
+  // the launches behind the first may be set up while the one before still runs
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(u.ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, extend_weights_kernel<KV>, c, u, w);
+  cfg.gridDim = dim3(static_cast<unsigned>(u.ptiles));
+  cfg.blockDim = dim3(kPos);
+  cfg.dynamicSmemBytes = 0;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, add_pieces_kernel, c, u, w);
+  if (e != cudaSuccess) { note_cuda_error(e, "extend_weights_kernel"); return AKL_ERR_CUDA; }
+  return AKL_OK;
+}
+
 }  // namespace
 }  // namespace akl
 
@@ -90,13 +532,26 @@ int akl_extend_weights(const akl_weights_t* c, void* stream) {
   akl_weights_layout_t L;
   int rc = check_weights(c, &L);
   if (rc != AKL_OK) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned blocks = (static_cast<unsigned>(c->N) + 7) / 8;
-  if (c->kv_dtype == AKL_KV_BF16) extend_weights_kernel<AKL_KV_BF16><<<blocks, 256, 0, s>>>(*c);
-  else extend_weights_kernel<AKL_KV_FP16><<<blocks, 256, 0, s>>>(*c);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) { note_cuda_error(e, "extend_weights_kernel"); return AKL_ERR_CUDA; }
-  return AKL_OK;
+  int sms = 0;
+  if ((rc = device_sm_count(&sms)) != AKL_OK) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(c->workspace);
+  Units u;
+  u.group = c->q_heads / c->kv_heads;
+  u.heads = c->kv_heads;
+  u.tiles = static_cast<int>((static_cast<int64_t>(c->T) * u.group + kRows - 1) / kRows);
+  u.ptiles = static_cast<int>((static_cast<int64_t>(c->N) + kPos - 1) / kPos);
+  u.prefix = c->prefix;
+  u.full = std::min(u.ptiles, c->prefix / kPos + 1);
+  u.total = u.start(u.ptiles);
+  u.ctas = std::min<long long>(std::min(sms, kMaxCtas), u.total);
+  Work w;
+  w.images = ws + L.off_q;
+  w.pos_cap = static_cast<int>((static_cast<int64_t>(c->plan.max_kv_len) + kPos - 1) / kPos * kPos);
+  w.sums = reinterpret_cast<float*>(ws + L.off_parts);
+  w.more = reinterpret_cast<float*>(ws + L.off_parts + align1k(static_cast<uint64_t>(w.pos_cap) * c->kv_heads * 4));
+  w.status = reinterpret_cast<int*>(ws + L.off_status);
+  return c->kv_dtype == AKL_KV_BF16 ? launch_weights<AKL_KV_BF16>(*c, u, w, ws + L.off_q, static_cast<cudaStream_t>(stream))
+                                    : launch_weights<AKL_KV_FP16>(*c, u, w, ws + L.off_q, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -149,7 +149,7 @@ class WeightsPlan(ctypes.Structure):
 
 
 class WeightsLayout(ctypes.Structure):
-    _fields_ = _fields("u64: total_bytes off_status off_q off_rows off_parts")
+    _fields_ = _fields("u64: total_bytes off_status off_q off_parts")
 
 
 class Weights(ctypes.Structure):

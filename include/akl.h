@@ -345,9 +345,8 @@ typedef struct akl_weights_plan {
 typedef struct akl_weights_layout {
   uint64_t total_bytes;       /* 1024-byte aligned base */
   uint64_t off_status;        /* [64] i32; word 0 = AKL_ERR_TIMEOUT if a bounded wait ran out */
-  uint64_t off_q;             /* Q rows packed by kv head, in the pool's type */
-  uint64_t off_rows;          /* per packed row {factor, lse} f32 */
-  uint64_t off_parts;         /* [parts][max_kv_len] f32 partial sums */
+  uint64_t off_q;             /* Q rows packed by kv head, in the pool's type, with their factors and lse */
+  uint64_t off_parts;         /* f32 partial sums */
 } akl_weights_layout_t;
 
 typedef struct akl_weights {
