@@ -41,7 +41,8 @@ constexpr int kPos = 256;                           // positions of a unit: two 
 constexpr int kImage = 4 * kPlaneBytes;             // four planes of 64 channels, 128-byte swizzle
 constexpr int kTileBytes = kImage + 2 * kRows * 4;  // and per row {factor}[128], {-lse}[128]
 constexpr int kStages = 3;
-constexpr int kEpiWarps = 8;
+constexpr int kPieceCost = 2;                       // units that bringing a K tile in takes the time of
+constexpr int kEpiWarps = 16;
 constexpr int kThreads = (kEpiWarps + 3) * 32;      // + two warps that issue products, one that fetches rows
 constexpr uint32_t kTmemCols = 512, kColD = 0, kColK = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -65,10 +66,11 @@ int weights_layout(const akl_weights_plan_t& p, akl_weights_layout_t* o) {
   return AKL_OK;
 }
 
-// The sequence of units, from the call alone.
+// The sequence of units, from the call alone.  A (position tile, kv head) costs its row tiles and
+// kPieceCost more for the K that has to come in first.
 struct Units {
   int group, heads, tiles, ptiles, full, prefix;    // full: position tiles that every row tile sees
-  long long total;
+  long long total;                                  // cost of everything
   long long ctas;
   __host__ __device__ int first_tile(int p) const { // row tiles before this one see nothing of position tile p
     const long long n0 = static_cast<long long>(p) * kPos - prefix;
@@ -78,10 +80,38 @@ struct Units {
     const int f = first_tile(p);
     return f < tiles ? tiles - f : 0;
   }
+  __host__ __device__ int cost(int p) const {
+    const int n = count(p);
+    return n > 0 ? n + kPieceCost : 0;
+  }
   __host__ __device__ long long start(int p) const {
-    long long u = static_cast<long long>(p < full ? p : full) * tiles;
-    for (int i = full; i < p; ++i) u += count(i);
+    long long u = static_cast<long long>(p < full ? p : full) * (tiles + kPieceCost);
+    for (int i = full; i < p; ++i) u += cost(i);
     return u * heads;
+  }
+  // Where cost `at` (below total) falls, and how many units lie before it.
+  __device__ __forceinline__ long long locate(long long at, int& p, int& j, int& skip) const {
+    const long long per = static_cast<long long>(heads) * (tiles + kPieceCost);
+    long long before;
+    if (at < per * full) {
+      p = static_cast<int>(at / per);
+      at -= per * p;
+      before = static_cast<long long>(p) * heads * tiles;
+    } else {
+      at -= per * full;
+      before = static_cast<long long>(full) * heads * tiles;
+      for (p = full; p + 1 < ptiles; ++p) {
+        const long long n = static_cast<long long>(heads) * cost(p);
+        if (at < n) break;
+        at -= n;
+        before += static_cast<long long>(heads) * count(p);
+      }
+    }
+    const int n = count(p), each = n + kPieceCost;
+    j = static_cast<int>(at / each);
+    skip = static_cast<int>(at - static_cast<long long>(j) * each) - kPieceCost;
+    skip = skip < 0 ? 0 : skip;
+    return before + static_cast<long long>(j) * n + skip;
   }
 };
 
@@ -128,7 +158,11 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const akl_weights_t c, u
       raw = make_uint4(pk[0], pk[1], pk[2], pk[3]);
     }
   }
-  *reinterpret_cast<uint4*>(image + (lane >> 3) * kPlaneBytes + swz128(row, (lane & 7) * 16)) = raw;
+  // words 4 q .. 4 q + 3 of every 16 go to 2 q, 2 q + 1, 8 + 2 q and 9 + 2 q, the order of K in TMEM
+  uint8_t* plane = image + (lane >> 3) * kPlaneBytes;
+  const int col = ((lane >> 2) & 1) * 64 + (lane & 3) * 8;
+  *reinterpret_cast<uint2*>(plane + swz128(row, col)) = make_uint2(raw.x, raw.y);
+  *reinterpret_cast<uint2*>(plane + swz128(row, col + 32)) = make_uint2(raw.z, raw.w);
   if (lane == 0) {
     float* f = reinterpret_cast<float*>(image + kImage);
     f[row] = factor;
@@ -145,8 +179,8 @@ struct Bars {
   __device__ uint32_t k_full() const { return base + (2 * kStages + 4) * 8; }
 };
 constexpr int kBars = 2 * kStages + 5;
-constexpr int kOffRed = kStages * kTileBytes;       // [2][kPos] floats, behind the row tiles
-constexpr int kOffBar = kOffRed + 2 * kPos * 4;
+constexpr int kOffRed = kStages * kTileBytes;       // [2][3][kPos] floats, behind the row tiles
+constexpr int kOffBar = kOffRed + 6 * kPos * 4;
 constexpr int kOffMisc = kOffBar + kBars * 8 + 8;
 constexpr int kSmem = kOffMisc + 64 + 1024;         // + alignment slack
 static_assert(kSmem <= 232448 && kTileBytes % 1024 == 0, "shared memory");
@@ -188,32 +222,40 @@ __device__ __forceinline__ void mma_16_ts(uint32_t d, uint32_t a, uint64_t b, ui
       : "memory");
 }
 
+// Sixteen TMEM lanes x 32 columns: thread (g, q) = (lane / 4, lane % 4) stores, of each group of eight
+// columns, columns 2 q, 2 q + 1 of lanes g (v[0], v[1]) and g + 8 (v[2], v[3]).
+__device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::AKL_I8(v, 0), AKL_I8(v, 8), "r"(taddr)
+      : "memory");
+}
+// Values of an asynchronous TMEM load exist from here on (behind its wait).
+__device__ __forceinline__ void pin32(uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));
+}
+
 // What this CTA's share holds next: position tile p, kv head j, row tiles [r, r_end).
 struct Piece {
   int p, j, r, r_end;
   bool begins;
 };
-__device__ __forceinline__ Piece first_piece(const Units& u, long long at, long long count) {
+// The CTA's first piece and the number of units in its share.
+__device__ __forceinline__ Piece first_piece(const Units& u, long long from, long long to, int& count) {
   Piece x;
-  const long long per = static_cast<long long>(u.heads) * u.tiles;
-  long long in;
-  if (at < per * u.full) {
-    x.p = static_cast<int>(at / per);
-    in = at - per * x.p;
+  int p, j, skip;
+  const long long begin = u.locate(from, x.p, x.j, skip);
+  if (to < u.total) {
+    int more;
+    count = static_cast<int>(u.locate(to, p, j, more) - begin);
   } else {
-    in = at - per * u.full;
-    for (x.p = u.full;; ++x.p) {
-      const long long n = static_cast<long long>(u.heads) * u.count(x.p);
-      if (in < n || x.p + 1 >= u.ptiles) break;
-      in -= n;
-    }
+    int last;
+    count = static_cast<int>(u.locate(u.total - 1, p, j, last) + 1 - begin);      // the sequence ends with a unit
   }
-  const int n = max(1, u.count(x.p));
-  x.j = static_cast<int>(in / n);
-  const int skip = static_cast<int>(in - static_cast<long long>(x.j) * n);
   x.begins = skip == 0;
   x.r = u.first_tile(x.p) + skip;
-  x.r_end = static_cast<int>(min(static_cast<long long>(u.tiles), x.r + count));
+  x.r_end = static_cast<int>(min(static_cast<long long>(u.tiles), static_cast<long long>(x.r) + count));
   return x;
 }
 // The piece behind x; `left` units of the share remain, at least one.
@@ -281,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
   const uint32_t tmem = *tmem_slot;
 
   const long long first = u.total * blockIdx.x / u.ctas;
-  const int count = static_cast<int>(u.total * (blockIdx.x + 1) / u.ctas - first);
-  const Piece begin = first_piece(u, first, count);
+  int count;
+  const Piece begin = first_piece(u, first, u.total * (blockIdx.x + 1) / u.ctas, count);
 
   if (warp >= kEpiWarps) {
     if (lane == 0) {
@@ -332,95 +374,105 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
       }
     }
   } else {
-    // ---- positions: lane set `warp & 3` of both halves of the tile, columns 64 (warp / 4) ..
+    // ---- positions: lane set `warp & 3` of both halves of the tile, columns 32 (warp / 4) ..  Four warps
+    // a scheduler: with two the exponential unit idled a third of the time behind their latencies.
     const int quarter = warp & 3, side = warp >> 2;
     const int at = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float factor = c.sm_scale * kLog2e;
     float* red = reinterpret_cast<float*>(smem_gen + kOffRed);
     Piece x = begin;
-    int it = 0, piece = 0;
+    int it = 0, piece = 0, slot_tile = -1;
+    long long slot = -1;             // of this lane's position in the tile
     bool ok = true;
     while (it < count) {
-      // K of position 128 side + at into TMEM.  Every product of the piece before has been waited for.
+      // K of 32 positions, channels 128 (side & 1) .., into TMEM.  Every product of the piece before has been
+      // waited for.  Four lanes share a row, so that a load of the warp reads 64 bytes of eight rows (a row
+      // per lane would be 32 lines a load); 16-lane stores put two words of a lane side by side, so the
+      // channels of a row lie in TMEM as pack_rows_kernel lays those of Q (a product does not mind their order).
       {
-        const long long n = static_cast<long long>(x.p) * kPos + side * 128 + at;
-        const uint4* src = nullptr;
-        if (n < c.N) {
-          const long long slot = load_index(c.idx, c.idx_dtype, n);
-          if (slot >= 0 && slot < c.pool_rows)
-            src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + x.j * 256);
+        const int sub = side >> 1, part = side & 1;
+        if (x.p != slot_tile) {
+          slot_tile = x.p;
+          const long long n = static_cast<long long>(x.p) * kPos + sub * 128 + at;
+          slot = -1;
+          if (n < c.N) slot = load_index(c.idx, c.idx_dtype, n);
+          if (slot >= c.pool_rows) slot = -1;
         }
         tc_fence_after();
 #pragma unroll
-        for (int part = 0; part < 4; part += 2) {
-          uint32_t v[2][32];
+        for (int b = 0; b < 2; ++b) {                  // positions 16 b .. of the warp's
+          uint32_t v[2][16];                           // [channels 64 ..][pairs of words: row, row + 8, ..]
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+          for (int e = 0; e < 2; ++e) {
+            const long long row = __shfl_sync(0xffffffffu, slot, b * 16 + e * 8 + (lane >> 2));
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k_pool) + (row < 0 ? 0 : row) * c.k_stride + x.j * 256) +
+                               part * 16 + (lane & 3);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint4 raw = src != nullptr ? __ldg(src + (part + b) * 8 + i) : make_uint4(0u, 0u, 0u, 0u);
-              v[b][4 * i] = raw.x;
-              v[b][4 * i + 1] = raw.y;
-              v[b][4 * i + 2] = raw.z;
-              v[b][4 * i + 3] = raw.w;
+            for (int i = 0; i < 4; ++i) {              // 64 bytes: two groups of eight columns
+              uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+              if (row >= 0) raw = __ldg(src + i * 4);
+              uint32_t* dst = &v[i >> 1][(i & 1) * 8 + e * 2];
+              dst[0] = raw.x;
+              dst[1] = raw.y;
+              dst[4] = raw.z;
+              dst[5] = raw.w;
             }
-          tmem_st32(lanes + kColK + side * 128 + part * 32, v[0]);
-          tmem_st32(lanes + kColK + side * 128 + part * 32 + 32, v[1]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tmem_st_16x256b_x4(tmem + (static_cast<uint32_t>(quarter * 32 + b * 16) << 16) + kColK + sub * 128 + part * 64 + i * 32, v[i]);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.k_full());
       }
+      // Packed rows from (n - prefix) group on see position n, and the last tile may be short.  Of 32
+      // columns against the warp's 32 positions nearly always all count or none.
       float sum[2] = {0.f, 0.f};
-      const long long n0 = static_cast<long long>(x.p) * kPos - c.prefix;     // first position, against row 0's diagonal
+      const long long n0 = static_cast<long long>(x.p) * kPos + quarter * 32 - c.prefix;   // the warp's first position, against row 0's diagonal
       for (; x.r < x.r_end; ++x.r, ++it) {
         const int s = it % kStages;
         if (ok) ok = wait(bars.q_full(s), (it / kStages) & 1);
-        const float* rows = reinterpret_cast<const float*>(smem_gen + s * kTileBytes + kImage) + side * 64;
+        const float* rows = reinterpret_cast<const float*>(smem_gen + s * kTileBytes + kImage) + side * 32;
+        const int col0 = x.r * kRows + side * 32, high = c.T * u.group - col0;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
           if (ok) ok = wait(bars.d_full(sub), it & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) continue;
           tc_fence_after();
-          uint32_t v[2][32];
-          tmem_ld32(lanes + kColD + sub * 128 + side * 64, v[0]);
-          tmem_ld32(lanes + kColD + sub * 128 + side * 64 + 32, v[1]);
+          uint32_t v[32];
+          tmem_ld32(lanes + kColD + sub * 128 + side * 32, v);
           tmem_wait_ld();
+          pin32(v);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars.d_empty(sub));
-          // packed rows from (n - prefix) group on see position n; the last tile may be short
-          const int tile0 = x.r * kRows + side * 64;
-          const int short_by = u.tiles * kRows - c.T * u.group;
-          const bool cut = (n0 + sub * 128 + 127) * u.group > x.r * kRows || (x.r + 1 == u.tiles && short_by > 0);
-          if (!cut) {
-            sum[sub] += add_columns<KV, false>(v[0], rows, factor, 0, 32) + add_columns<KV, false>(v[1], rows + 32, factor, 0, 32);
-          } else {
-            const long long low = (n0 + sub * 128 + at) * u.group - tile0;
-            const int lo = static_cast<int>(max(-64ll, min(64ll, low)));
-            const int hi = min(64, c.T * u.group - tile0);
-            sum[sub] += add_columns<KV, true>(v[0], rows, factor, lo, hi) + add_columns<KV, true>(v[1], rows + 32, factor, lo - 32, hi - 32);
-          }
+          const int first = static_cast<int>(max(-4096ll, min(4096ll, (n0 + sub * 128) * u.group - col0))), last = first + 31 * u.group;
+          if (last <= 0 && high >= 32) sum[sub] += add_columns<KV, false>(v, rows, factor, 0, 32);
+          else if (first < 32 && high > 0) sum[sub] += add_columns<KV, true>(v, rows, factor, first + lane * u.group, high);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.q_empty(s));
       }
-      // the two halves of the columns meet; a piece's buffer is used again two pieces, so one barrier, later
+      // the four quarters of the columns meet; a piece's buffer is used again two pieces, so one barrier, later
       if (!ok) sum[0] = sum[1] = __int_as_float(0x7FC00000);
-      float* meet = red + (piece & 1) * kPos;
-      if (side == 1) {
-        meet[at] = sum[0];
-        meet[128 + at] = sum[1];
+      float* meet = red + (piece & 1) * 3 * kPos;
+      if (side > 0) {
+        meet[(side - 1) * kPos + at] = sum[0];
+        meet[(side - 1) * kPos + 128 + at] = sum[1];
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
       if (side == 0) {
         float* dst = x.begins ? w.sums + static_cast<long long>(x.j) * w.pos_cap + static_cast<long long>(x.p) * kPos
                               : w.more + static_cast<long long>(blockIdx.x) * kPos;
-        dst[at] = sum[0] + meet[at];
-        dst[128 + at] = sum[1] + meet[128 + at];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          const float* m = meet + sub * 128 + at;
+          dst[sub * 128 + at] = (sum[sub] + m[0]) + (m[kPos] + m[2 * kPos]);
+        }
       }
       ++piece;
       if (it < count) x = next_piece(u, x, count - it);
@@ -449,7 +501,7 @@ __global__ void __launch_bounds__(kPos) add_pieces_kernel(const akl_weights_t c,
   if (n >= c.N) return;
   float total = 0.f;
   for (int j = 0; units > 0 && there && j < u.heads; ++j) {
-    const long long at = base + static_cast<long long>(j) * units;
+    const long long at = base + static_cast<long long>(j) * (units + kPieceCost) + kPieceCost;   // the first unit
     float v = w.sums[static_cast<long long>(j) * w.pos_cap + n];
     // CTAs whose share begins inside (at, at + units)
     const long long lo = ((at + 1) * u.ctas + u.total - 1) / u.total;
