@@ -34,14 +34,13 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kMaxGroup = 8;
+constexpr int kMaxGroup = 8, kMaxHeads = 8;         // q heads per kv head, kv heads
 constexpr int kMaxCtas = 160;
 constexpr int kRows = 128;                          // packed rows of a tile
 constexpr int kPos = 256;                           // positions of a unit: two TMEM lane sets
 constexpr int kImage = 4 * kPlaneBytes;             // four planes of 64 channels, 128-byte swizzle
 constexpr int kTileBytes = kImage + 2 * kRows * 4;  // and per row {factor}[128], {-lse}[128]
 constexpr int kStages = 3;
-constexpr int kPieceCost = 2;                       // units that bringing a K tile in takes the time of
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = (kEpiWarps + 3) * 32;      // + two warps that issue products, one that fetches rows
 constexpr uint32_t kTmemCols = 512, kColD = 0, kColK = 256;
@@ -67,9 +66,10 @@ int weights_layout(const akl_weights_plan_t& p, akl_weights_layout_t* o) {
 }
 
 // The sequence of units, from the call alone.  A (position tile, kv head) costs its row tiles and
-// kPieceCost more for the K that has to come in first.
+// `piece` more for the K that has to come in first.
 struct Units {
   int group, heads, tiles, ptiles, full, prefix;    // full: position tiles that every row tile sees
+  int piece;
   long long total;                                  // cost of everything
   long long ctas;
   __host__ __device__ int first_tile(int p) const { // row tiles before this one see nothing of position tile p
@@ -82,16 +82,16 @@ struct Units {
   }
   __host__ __device__ int cost(int p) const {
     const int n = count(p);
-    return n > 0 ? n + kPieceCost : 0;
+    return n > 0 ? n + piece : 0;
   }
   __host__ __device__ long long start(int p) const {
-    long long u = static_cast<long long>(p < full ? p : full) * (tiles + kPieceCost);
+    long long u = static_cast<long long>(p < full ? p : full) * (tiles + piece);
     for (int i = full; i < p; ++i) u += cost(i);
     return u * heads;
   }
   // Where cost `at` (below total) falls, and how many units lie before it.
   __device__ __forceinline__ long long locate(long long at, int& p, int& j, int& skip) const {
-    const long long per = static_cast<long long>(heads) * (tiles + kPieceCost);
+    const long long per = static_cast<long long>(heads) * (tiles + piece);
     long long before;
     if (at < per * full) {
       p = static_cast<int>(at / per);
@@ -107,9 +107,9 @@ struct Units {
         before += static_cast<long long>(heads) * count(p);
       }
     }
-    const int n = count(p), each = n + kPieceCost;
+    const int n = count(p), each = n + piece;
     j = static_cast<int>(at / each);
-    skip = static_cast<int>(at - static_cast<long long>(j) * each) - kPieceCost;
+    skip = static_cast<int>(at - static_cast<long long>(j) * each) - piece;
     skip = skip < 0 ? 0 : skip;
     return before + static_cast<long long>(j) * n + skip;
   }
@@ -123,50 +123,66 @@ struct Work {
   int pos_cap;               // positions between two kv heads of sums
 };
 
-// One warp per packed row: its image row in the pool's type, factor and -lse.
+// One CTA per tile of packed rows, a warp every 16 of them: image rows in the pool's type, factors and -lse.
 template <int KV>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const akl_weights_t c, uint8_t* images, int tiles) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int group = c.q_heads / c.kv_heads, j = blockIdx.y, lane = threadIdx.x & 31;
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), tile = r / kRows, row = r % kRows;
-  uint8_t* image = images + (static_cast<long long>(j) * tiles + tile) * kTileBytes;
-  const int t = r / group, h = j * group + r - t * group;
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  float factor = 0.f, neg = -INFINITY;
-  if (t < c.T) {
-    raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + t * c.q_stride + h * 256 + lane * 8);
-    factor = c.sm_scale * kLog2e;
-    const float lse = __ldg(c.lse + static_cast<long long>(t) * c.q_heads + h);
-    neg = isinf(lse) ? -INFINITY : -lse;             // a row that saw no key adds nothing
-    if (KV == AKL_KV_FP16) {
-      float x[8], top = 0.f;
-      unpack8<AKL_KV_BF16>(raw, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-      top = warp_max(top);
-      // 2^e <= top < 2^(e+1), with both 2^e and 2^-e normal; 1 for a row of zeros or of infinities
-      int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xFFu) - 127;
-      e = (top == 0.f || e == 128) ? 0 : max(-126, min(126, e));
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      uint32_t pk[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 v = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
-        pk[i] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-      raw = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-    }
-  }
+  const int row0 = (threadIdx.x >> 5) * 16, r0 = blockIdx.x * kRows + row0;
+  uint8_t* image = images + (static_cast<long long>(j) * tiles + blockIdx.x) * kTileBytes;
   // words 4 q .. 4 q + 3 of every 16 go to 2 q, 2 q + 1, 8 + 2 q and 9 + 2 q, the order of K in TMEM
   uint8_t* plane = image + (lane >> 3) * kPlaneBytes;
   const int col = ((lane >> 2) & 1) * 64 + (lane & 3) * 8;
-  *reinterpret_cast<uint2*>(plane + swz128(row, col)) = make_uint2(raw.x, raw.y);
-  *reinterpret_cast<uint2*>(plane + swz128(row, col + 32)) = make_uint2(raw.z, raw.w);
-  if (lane == 0) {
-    float* f = reinterpret_cast<float*>(image + kImage);
-    f[row] = factor;
-    f[kRows + row] = neg;
+  int t = r0 / group, h = r0 - t * group;
+#pragma unroll 1
+  for (int half = 0; half < 16; half += 8) {
+    uint4 raw[8];
+    float lse[8];
+    int tt = t, hh = h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      lse[i] = INFINITY;
+      if (tt < c.T) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.q) + tt * c.q_stride + (j * group + hh) * 256 + lane * 8));
+        lse[i] = __ldg(c.lse + static_cast<long long>(tt) * c.q_heads + j * group + hh);
+      }
+      if (++hh == group) { hh = 0; ++tt; }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + half + i;
+      float factor = c.sm_scale * kLog2e;
+      uint4 out = raw[i];
+      if (KV == AKL_KV_FP16) {
+        float x[8], top = 0.f;
+        unpack8<AKL_KV_BF16>(raw[i], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        top = warp_max(top);
+        // 2^e <= top < 2^(e+1), with both 2^e and 2^-e normal; 1 for a row of zeros or of infinities
+        int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xFFu) - 127;
+        e = (top == 0.f || e == 128) ? 0 : max(-126, min(126, e));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        uint32_t pk[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __half2 v = __floats2half2_rn(x[2 * k] * down, x[2 * k + 1] * down);
+          pk[k] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        out = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+      }
+      *reinterpret_cast<uint2*>(plane + swz128(row, col)) = make_uint2(out.x, out.y);
+      *reinterpret_cast<uint2*>(plane + swz128(row, col + 32)) = make_uint2(out.z, out.w);
+      if (lane == 0) {
+        float* f = reinterpret_cast<float*>(image + kImage);
+        f[row] = factor;
+        f[kRows + row] = isinf(lse[i]) ? -INFINITY : -lse[i];      // a row that saw no key, or is none, adds nothing
+      }
+    }
+    for (int i = 0; i < 8; ++i)
+      if (++h == group) { h = 0; ++t; }
   }
 }
 
@@ -267,7 +283,9 @@ __device__ __forceinline__ Piece next_piece(const Units& u, Piece x, long long l
   return x;
 }
 
-// 2^(s factor - lse) of 32 columns, added up; columns outside [low, high) count nothing.
+// 2^(s factor - lse) of 32 columns, added up; columns outside [low, high) count nothing.  The exponential
+// unit is busy 75 % of the time, as the tensor pipe is.  (Every fourth pair, or every eighth, as a polynomial
+// on the FMA pipe was measured: 172 us became 179 and 173, the issue slots then bind.)
 template <int KV, bool kMask>
 __device__ __forceinline__ float add_columns(const uint32_t (&v)[32], const float* rows, float factor, int low, int high) {
   f2 acc[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
@@ -382,8 +400,15 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
     const float factor = c.sm_scale * kLog2e;
     float* red = reinterpret_cast<float*>(smem_gen + kOffRed);
     Piece x = begin;
-    int it = 0, piece = 0, slot_tile = -1;
+    int it = 0, piece = 0, slot_tile = -1, stage = 0;
+    uint32_t q_phase = 0;
     long long slot = -1;             // of this lane's position in the tile
+    auto slot_of = [&](int p, int sub) {
+      const long long n = static_cast<long long>(p) * kPos + sub * 128 + at;
+      long long v = -1;
+      if (n < c.N) v = load_index(c.idx, c.idx_dtype, n);
+      return v < c.pool_rows ? v : -1ll;
+    };
     bool ok = true;
     while (it < count) {
       // K of 32 positions, channels 128 (side & 1) .., into TMEM.  Every product of the piece before has been
@@ -394,10 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
         const int sub = side >> 1, part = side & 1;
         if (x.p != slot_tile) {
           slot_tile = x.p;
-          const long long n = static_cast<long long>(x.p) * kPos + sub * 128 + at;
-          slot = -1;
-          if (n < c.N) slot = load_index(c.idx, c.idx_dtype, n);
-          if (slot >= c.pool_rows) slot = -1;
+          slot = slot_of(x.p, sub);
         }
         tc_fence_after();
 #pragma unroll
@@ -427,16 +449,38 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.k_full());
+        // the next piece's rows (a lane's own, two lines of this warp's channels) on their way to L2
+        const int left = count - it - (x.r_end - x.r);
+        if (left > 0) {
+          const Piece y = next_piece(u, x, left);
+          if (y.p != slot_tile) {
+            slot_tile = y.p;
+            slot = slot_of(y.p, sub);
+          }
+          if (slot >= 0) {
+            const uint16_t* row = static_cast<const uint16_t*>(c.k_pool) + slot * c.k_stride + y.j * 256 + part * 128;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(row));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(row + 64));
+          }
+        }
       }
       // Packed rows from (n - prefix) group on see position n, and the last tile may be short.  Of 32
       // columns against the warp's 32 positions nearly always all count or none.
       float sum[2] = {0.f, 0.f};
-      const long long n0 = static_cast<long long>(x.p) * kPos + quarter * 32 - c.prefix;   // the warp's first position, against row 0's diagonal
-      for (; x.r < x.r_end; ++x.r, ++it) {
-        const int s = it % kStages;
-        if (ok) ok = wait(bars.q_full(s), (it / kStages) & 1);
-        const float* rows = reinterpret_cast<const float*>(smem_gen + s * kTileBytes + kImage) + side * 32;
-        const int col0 = x.r * kRows + side * 32, high = c.T * u.group - col0;
+      int low[2], clear[2];            // first packed row that the warp's first position sees; first that all of them see
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const long long n0 = static_cast<long long>(x.p) * kPos + sub * 128 + quarter * 32 - c.prefix;
+        low[sub] = static_cast<int>(max(-(1ll << 29), min(1ll << 30, n0 * u.group)));
+        clear[sub] = low[sub] + 31 * u.group;
+      }
+      const int packed = c.T * u.group;
+      int col0 = x.r * kRows + side * 32;
+      const uint32_t d_lanes = lanes + kColD + side * 32;
+#pragma unroll 1
+      for (; x.r < x.r_end; ++x.r, ++it, col0 += kRows) {
+        if (ok) ok = wait(bars.q_full(stage), q_phase);
+        const float* rows = reinterpret_cast<const float*>(smem_gen + stage * kTileBytes + kImage) + side * 32;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
           if (ok) ok = wait(bars.d_full(sub), it & 1);
@@ -444,18 +488,18 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
           if (!ok) continue;
           tc_fence_after();
           uint32_t v[32];
-          tmem_ld32(lanes + kColD + sub * 128 + side * 32, v);
+          tmem_ld32(d_lanes + sub * 128, v);
           tmem_wait_ld();
           pin32(v);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars.d_empty(sub));
-          const int first = static_cast<int>(max(-4096ll, min(4096ll, (n0 + sub * 128) * u.group - col0))), last = first + 31 * u.group;
-          if (last <= 0 && high >= 32) sum[sub] += add_columns<KV, false>(v, rows, factor, 0, 32);
-          else if (first < 32 && high > 0) sum[sub] += add_columns<KV, true>(v, rows, factor, first + lane * u.group, high);
+          if (col0 + 32 <= packed && clear[sub] <= col0) sum[sub] += add_columns<KV, false>(v, rows, factor, 0, 32);
+          else if (low[sub] < col0 + 32) sum[sub] += add_columns<KV, true>(v, rows, factor, low[sub] + lane * u.group - col0, packed - col0);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.q_empty(s));
+        if (lane == 0) mbar_arrive(bars.q_empty(stage));
+        if (++stage == kStages) { stage = 0; q_phase ^= 1; }
       }
       // the four quarters of the columns meet; a piece's buffer is used again two pieces, so one barrier, later
       if (!ok) sum[0] = sum[1] = __int_as_float(0x7FC00000);
@@ -488,28 +532,38 @@ __global__ void __launch_bounds__(kThreads, 1) extend_weights_kernel(const akl_w
 
 // One CTA per position tile: heads in order, of each the piece that begins it and those that go on.
 __global__ void __launch_bounds__(kPos) add_pieces_kernel(const akl_weights_t c, const Units u, const Work w) {
+  __shared__ int sm_from[kMaxHeads], sm_to[kMaxHeads];
   const int p = blockIdx.x;
   const long long n = static_cast<long long>(p) * kPos + threadIdx.x;
   const int units = u.count(p);
-  const long long base = u.start(p);
+  if (threadIdx.x < u.heads) {
+    // CTAs whose share begins behind the first unit of (p, head): floor(total i / ctas) in [at + 1, at + units)
+    const long long at = u.start(p) + static_cast<long long>(threadIdx.x) * (units + u.piece) + u.piece;
+    sm_from[threadIdx.x] = static_cast<int>(((at + 1) * u.ctas + u.total - 1) / u.total);
+    sm_to[threadIdx.x] = static_cast<int>(min(u.ctas, ((at + units) * u.ctas + u.total - 1) / u.total));
+  }
   bool there = false;
   if (n < c.N) {
     const long long slot = load_index(c.idx, c.idx_dtype, n);
     there = slot >= 0 && slot < c.pool_rows;
   }
+  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (n >= c.N) return;
-  float total = 0.f;
-  for (int j = 0; units > 0 && there && j < u.heads; ++j) {
-    const long long at = base + static_cast<long long>(j) * (units + kPieceCost) + kPieceCost;   // the first unit
-    float v = w.sums[static_cast<long long>(j) * w.pos_cap + n];
-    // CTAs whose share begins inside (at, at + units)
-    const long long lo = ((at + 1) * u.ctas + u.total - 1) / u.total;
-    const long long hi = min(u.ctas, ((at + units) * u.ctas + u.total - 1) / u.total);
-    for (long long i = lo; i < hi; ++i) v += w.more[i * kPos + threadIdx.x];
-    total += v;
+  const float old = c.weight_decay == 0.f ? 0.f : c.weights[n];
+  float part[kMaxHeads];
+#pragma unroll
+  for (int j = 0; j < kMaxHeads; ++j) {
+    part[j] = 0.f;
+    if (j < u.heads && units > 0 && there) {
+      part[j] = w.sums[static_cast<long long>(j) * w.pos_cap + n];
+      for (int i = sm_from[j]; i < sm_to[j]; ++i) part[j] += w.more[static_cast<long long>(i) * kPos + threadIdx.x];
+    }
   }
-  c.weights[n] = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, c.weights[n], total);
+  float total = 0.f;
+#pragma unroll
+  for (int j = 0; j < kMaxHeads; ++j) total += part[j];
+  c.weights[n] = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, old, total);
 }
 
 int check_weights(const akl_weights_t* c, akl_weights_layout_t* L) {
@@ -545,7 +599,7 @@ int launch_weights(const akl_weights_t& c, const Units& u, const Work& w, uint8_
     if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
   if (e == cudaSuccess) {
-    pack_rows_kernel<KV><<<dim3(u.tiles * (kRows / 8), c.kv_heads), 256, 0, s>>>(c, images, u.tiles);
+    pack_rows_kernel<KV><<<dim3(u.tiles, c.kv_heads), 256, 0, s>>>(c, images, u.tiles);
     e = cudaGetLastError();
   }
   // the launches behind the first may be set up while the one before still runs
@@ -594,8 +648,16 @@ int akl_extend_weights(const akl_weights_t* c, void* stream) {
   u.ptiles = static_cast<int>((static_cast<int64_t>(c->N) + kPos - 1) / kPos);
   u.prefix = c->prefix;
   u.full = std::min(u.ptiles, c->prefix / kPos + 1);
+  // A K tile takes about four units' time to come in, which counts where row tiles are many: beside the
+  // diagonal a share then has up to ten pieces, elsewhere two.  (2048 rows, 8192 before them: 180 us at
+  // 2, 172 at 4, 170 at 6; with few units a share would be a K tile and no row to go with it.)
+  u.piece = 0;
   u.total = u.start(u.ptiles);
   u.ctas = std::min<long long>(std::min(sms, kMaxCtas), u.total);
+  if (u.total >= 16 * u.ctas) {
+    u.piece = 4;
+    u.total = u.start(u.ptiles);
+  }
   Work w;
   w.images = ws + L.off_q;
   w.pos_cap = static_cast<int>((static_cast<int64_t>(c->plan.max_kv_len) + kPos - 1) / kPos * kPos);
