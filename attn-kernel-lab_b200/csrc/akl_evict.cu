@@ -1,56 +1,65 @@
 // Eviction by accumulated weight: the first and last positions of a request and the heaviest of the
 // others move to the front of its page-table row in position order.
 //
-// The weights are compared as 32-bit keys in the order of the floats (NaN as -inf, -0 as 0).  The key
-// of the lightest position that stays is found digit by digit, eight bits a pass, from a histogram of
-// the keys that share the digits found so far; of the positions with exactly that key the lowest stay.
+// The weights are compared as 32-bit keys in the order of the floats (NaN as -inf, -0 as 0).  The key of
+// the lightest position that stays is found digit by digit -- 11, 11 and 10 bits -- from histograms of the
+// keys that share the digits found so far; of the positions with exactly that key the lowest stay.  The
+// new place of a position then follows from two counts, of the positions before it that stay for
+// certain and of those with that key.
+//
+// A CTA, or a cluster of them while the requests leave SMs idle, takes a request; a thread holds up to 32 of its
+// weights in registers, so a row that fits is read once and written once, whatever the passes.  The
+// histograms and counts of a cluster meet through its shared memory.  Longer rows go through in rounds, their
+// weights read again for each digit (from L2).  Rows may be shortened in place: positions only move forward,
+// and what a group of 8192 positions a CTA overwrites has been read by all when its barrier opens.
+//
+// Few bytes and two or three dependent passes: bound by the latency of the passes where requests are few, and
+// by the instructions per position where they are many, so the loops over a thread's positions have no branches.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <atomic>
+
 #include "akl_common.cuh"
 
 namespace akl {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kStep = 8, kGroups = 4;           // positions of a thread: groups of up to eight
+constexpr int kCap = kThreads * kStep * kGroups;
+constexpr int kMaxCluster = 16;
+constexpr int kBins = 2048;
+
+constexpr uint32_t kStays = 0xFFFFFFFFu;      // key of a position that stays whatever its weight; above every weight's
+constexpr uint32_t kNothing = 0u;              // key where there is no position; below every weight's
 
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) w = -INFINITY;
-  w = w + 0.f;
-  const uint32_t u = __float_as_uint(w);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint((w != w ? -INFINITY : w) + 0.f);
+  return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_weight(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// Exclusive count of `flag` before this thread in the CTA, and the total.
-__device__ __forceinline__ int cta_rank(bool flag, int* sm, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned ballot = __ballot_sync(0xffffffffu, flag);
-  if (lane == 0) sm[warp] = __popc(ballot);
-  __syncthreads();
-  if (warp == 0) {
-    const int v = sm[lane];
-    int s = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += up;
-    }
-    sm[lane] = s - v;
-    if (lane == 31) sm[32] = s;
-  }
-  __syncthreads();
-  const int rank = sm[warp] + __popc(ballot & ((1u << lane) - 1u));
-  total = sm[32];
-  __syncthreads();
-  return rank;
-}
+struct Shared {
+  int hist[3][kBins];
+  int4 found[3];                   // of each pass, in the cluster's first CTA: digit, how many of it stay, whether all
+  uint32_t counts[kGroups][kWarps];  // certain | equal << 16
+  uint32_t totals[2][kGroups];     // of this CTA, by parity of the round; read by the cluster
+  int warp_sums[kWarps];
+};
 
-// One CTA per request.
 template <typename Slot>
-__global__ void __launch_bounds__(kThreads) evict_kernel(akl_evict_t c) {
-  __shared__ int sm_scan[33];
-  __shared__ int hist[256];
-  __shared__ uint32_t sm_prefix;
-  __shared__ int sm_need;
-  const int b = blockIdx.x, tid = threadIdx.x;
+__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c) {
+  __shared__ __align__(16) Shared sm;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned before = (1u << lane) - 1u;
   const long long row = c.rows != nullptr ? load_index(c.rows, c.rows_dtype, b) : b;
   long long len = load_index(c.kv_lens, c.lens_dtype, b);
   len = len < 0 ? 0 : (len > c.table_width ? c.table_width : len);
@@ -62,58 +71,273 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(akl_evict_t c) {
   Slot* slots_out = static_cast<Slot*>(c.page_table_out) + row * c.table_out_stride;
   float* weights_out = c.weights_out + row * c.weights_out_stride;
   Slot* freed = static_cast<Slot*>(c.freed) + b * c.freed_stride;
+  const int low = full ? c.first : n, high = full ? n - c.last : n;   // positions [low, high) compete, the others stay
+  int need = c.keep;                                    // places for them all
+  const bool idle = !full && slots_out == slots && weights_out == weights;   // nothing to move
+  const int per_round = ctas * kCap;
+  const bool once = n <= per_round;
+  auto key_of = [&](float w, int i) { return i >= n ? kNothing : (i < low || i >= high ? kStays : weight_key(w)); };
 
-  uint32_t threshold = 0;
-  int need = c.keep - c.first - c.last;         // how many of the middle stay
-  if (full && need > 0) {
-    if (tid == 0) { sm_prefix = 0; sm_need = need; }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      const uint32_t prefix = sm_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int i = c.first + tid; i < n - c.last; i += kThreads) {
-        const uint32_t k = weight_key(weights[i]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+  // A group is side by side in the row, in it a CTA's share, in it a warp's: `each` steps of 32 positions.
+  uint32_t key[kGroups][kStep];
+  int each = 0, groups = 0, base = 0;
+  unsigned alike = 0, odd = 0;                          // groups of which the warp's keys are all one; some are not the weight's bits
+  auto start_of = [&](int g) { return base + ((g * ctas + rank) * kWarps + warp) * each * 32 + lane; };
+  auto load = [&]() {
+    const int left = min(per_round, n - base), wide = (left + ctas * kThreads - 1) / (ctas * kThreads);
+    each = min(kStep, wide);
+    groups = (wide + each - 1) / each;
+    alike = odd = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)                   // the weights' bits first, so that all the loads are in flight
+      if (g < groups) {
+        const int at = start_of(g);
+        const float* from = weights + at;
+        if (each == kStep && at - lane + kStep * 32 <= n) {
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) key[g][k] = __float_as_uint(from[k * 32]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) key[g][k] = k < each && at + k * 32 < n ? __float_as_uint(from[k * 32]) : 0u;
+        }
+        // the slots are wanted behind the passes: have them in L2 by then
+        const int line = at - lane + lane * static_cast<int>(128 / sizeof(Slot));
+        if (lane * static_cast<int>(128 / sizeof(Slot)) < each * 32 && line < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(slots + line));
       }
-      __syncthreads();
-      if (tid == 0) {
-        int left = sm_need, d = 255;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        sm_need = left;
-        sm_prefix = prefix | (static_cast<uint32_t>(d) << shift);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if (g < groups) {
+        const int at = start_of(g), from = at - lane, to = from + each * 32;
+        uint32_t least = key[g][0], most = key[g][0];
+#pragma unroll
+        for (int k = 1; k < kStep; ++k) {
+          least = min(least, key[g][k]);
+          most = max(most, key[g][k]);
+        }
+        // weights that are at least 0 and no NaN, in positions that compete, are their own order
+        if (__all_sync(0xffffffffu, most <= 0x7F800000u) && from >= low && to <= high && each == kStep) {
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) key[g][k] |= 0x80000000u;
+          const uint32_t first = __shfl_sync(0xffffffffu, least, 0);
+          if (__all_sync(0xffffffffu, least == first && most == first)) alike |= 1u << g;
+        } else {
+          bool strange = false, same = true;
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const uint32_t bits = key[g][k];
+            key[g][k] = k < each ? key_of(__uint_as_float(bits), at + k * 32) : kNothing;
+            strange |= key[g][k] != kNothing && __float_as_uint(key_weight(key[g][k])) != bits;
+          }
+          const uint32_t first = __shfl_sync(0xffffffffu, key[g][0], 0);
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) same &= key[g][k] == first || k >= each;
+          if (__all_sync(0xffffffffu, same)) alike |= 1u << g;
+          if (__any_sync(0xffffffffu, strange)) odd |= 1u << g;
+        }
       }
-      __syncthreads();
-    }
-    threshold = sm_prefix;
-    need = sm_need;                             // how many of those with exactly this key stay
-  }
-  int stay0 = 0, go0 = 0, equal0 = 0;
-  for (int base = 0; base < n; base += kThreads) {
-    const int i = base + tid;
-    const bool in = i < n;
-    const bool middle = in && full && i >= c.first && i < n - c.last;
-    const Slot slot = in ? slots[i] : Slot(0);
-    const float w = in ? weights[i] : 0.f;
-    const uint32_t key = weight_key(w);
-    const bool equal = middle && key == threshold;
-    int total;
-    const int rank = cta_rank(equal, sm_scan, total);
-    const bool stay = in && (!middle || (c.keep > c.first + c.last && (key > threshold || (equal && equal0 + rank < need))));
-    equal0 += total;
-    const int at = cta_rank(stay, sm_scan, total);      // ends with a barrier: the chunk is in registers
-    if (stay) { slots_out[stay0 + at] = slot; weights_out[stay0 + at] = w; }
-    const int before = min(tid, n - base) - at;
-    if (in && !stay) freed[go0 + before] = slot;
-    stay0 += total;
-    go0 += min(kThreads, n - base) - total;
+  };
+  if (!idle && n > 0 && once) load();
+
+  uint32_t threshold = kStays;
+  if (full) {
+    for (int i = tid; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<int4*>(sm.hist)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
+    if (ctas > 1) cluster.barrier_arrive();             // waited for before anybody adds to the first CTA's counts
+    uint32_t prefix = 0;
+    bool exact = false;                                 // every key that begins with prefix stays
+    for (int pass = 0; pass < 3 && !exact; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+      int* hist = sm.hist[pass];
+      const uint32_t mask = (1u << bits) - 1u;
+      auto add = [&](uint32_t k) {
+        const uint32_t d = k >> shift;
+        if (pass == 0 ? k != kNothing : (d >> bits) == prefix) atomicAdd(&hist[d & mask], 1);
+      };
+      if (once) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          if (g < groups) {
+            if ((alike >> g) & 1u) {
+              // one key (of weights that nobody has added to yet): one lane adds for all, or 32 would queue
+              const uint32_t d = key[g][0] >> shift;
+              if (lane == 0 && (pass == 0 ? key[g][0] != kNothing : (d >> bits) == prefix)) atomicAdd(&hist[d & mask], 32 * each);
+            } else {
+#pragma unroll
+              for (int k = 0; k < kStep; ++k) add(key[g][k]);
+            }
+          }
+      } else {
+        const int step = ctas * kThreads;
+        for (int at = rank * kThreads + tid; at < n; at += kStep * step) {
+          float v[kStep];
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) v[k] = at + k * step < n ? weights[at + k * step] : 0.f;
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) add(key_of(v[k], at + k * step));
+        }
+      }
+      // the cluster's counts meet in its first CTA, which finds the digit for all
+      __syncthreads();
+      if (ctas > 1) {
+        if (pass == 0) cluster.barrier_wait();
+        if (rank > 0) {
+          int* to = cluster.map_shared_rank(hist, 0);
+          const int2 mine = reinterpret_cast<const int2*>(hist)[tid];
+          if (mine.x != 0) atomicAdd(to + 2 * tid, mine.x);
+          if (mine.y != 0) atomicAdd(to + 2 * tid + 1, mine.y);
+        }
+        cluster.sync();
+      }
+      if (rank == 0) {
+        // bins from the top down, two a thread: the one in which the need-th heaviest lies
+        const int top = kBins - 2 - 2 * tid;            // its bins are top + 1, top
+        const int2 mine = *reinterpret_cast<const int2*>(hist + top);
+        const int sum = mine.x + mine.y;
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += v;
+        }
+        if (lane == 31) sm.warp_sums[warp] = upto;
+        __syncthreads();
+        upto += __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_sums[lane] : 0);
+        if (upto >= need && upto - sum < need) {        // one thread
+          const int left = need - (upto - sum);
+          sm.found[pass] = left > mine.y ? make_int4(top, left - mine.y, left - mine.y == mine.x, 0) : make_int4(top + 1, left, left == mine.y, 0);
+        }
+      }
+      if (ctas > 1) cluster.sync();
+      else __syncthreads();
+      const int4 found = *cluster.map_shared_rank(&sm.found[pass], 0);
+      prefix = (prefix << bits) | static_cast<uint32_t>(found.x);
+      need = found.y;
+      exact = found.z != 0;
+      threshold = prefix << shift;
+    }
+    if (exact) need = 0x7fffffff;                       // a whole bin stays: above its lower end, or equal to it
+  } else {
+    need = 0x7fffffff;
   }
-  for (int i = stay0 + tid; i < n; i += kThreads) weights_out[i] = 0.f;
-  if (tid == 0) {
-    if (c.lens_dtype == AKL_IDX_I64) static_cast<long long*>(c.kv_lens_out)[b] = stay0;
-    else static_cast<int*>(c.kv_lens_out)[b] = stay0;
-    c.freed_lens[b] = go0;
+  const bool in_place = static_cast<const void*>(slots_out) == static_cast<const void*>(slots);
+
+  int certain0 = 0, equal0 = 0;                         // in the groups before
+  for (int round = 0; base < n && !idle; base += per_round, ++round) {
+    if (!once) load();
+    uint32_t mine[kGroups];                             // of this warp: certain | equal << 16
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if (g < groups) {
+        uint32_t count = 0;
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) count += (key[g][k] > threshold ? 1u : 0u) + (key[g][k] == threshold ? 0x10000u : 0u);
+        mine[g] = __reduce_add_sync(0xffffffffu, count);
+        if (lane == 0) sm.counts[g][warp] = mine[g];
+      }
+    __syncthreads();
+    if (ctas > 1) {
+      if (warp < groups) {
+        const uint32_t total = __reduce_add_sync(0xffffffffu, sm.counts[warp][lane]);
+        if (lane == 0) sm.totals[round & 1][warp] = total;
+      }
+      cluster.sync();                                   // every weight of the round is in a register
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if (g < groups) {
+        const int at = start_of(g);
+        Slot slot[kStep];
+        float w[kStep];
+        const bool again = ((odd >> g) & 1u) != 0u;
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+          w[k] = key_weight(key[g][k]);
+          if (key[g][k] != kNothing) {
+            slot[k] = slots[at + k * 32];
+            if (again) w[k] = weights[at + k * 32];
+          }
+        }
+        const uint32_t count = sm.counts[g][lane];
+        const uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < warp ? count : 0u);
+        int certain = certain0 + static_cast<int>(ahead & 0xFFFFu), equal = equal0 + static_cast<int>(ahead >> 16);
+        if (ctas > 1) {
+          // sums over a cluster pass 16 bits: certain and equal apart
+          const uint32_t theirs = lane < ctas ? *cluster.map_shared_rank(&sm.totals[round & 1][g], lane < ctas ? lane : 0) : 0u;
+          const int theirs_c = static_cast<int>(theirs & 0xFFFFu), theirs_e = static_cast<int>(theirs >> 16);
+          certain += __reduce_add_sync(0xffffffffu, lane < rank ? theirs_c : 0);
+          equal += __reduce_add_sync(0xffffffffu, lane < rank ? theirs_e : 0);
+          certain0 += __reduce_add_sync(0xffffffffu, theirs_c);
+          equal0 += __reduce_add_sync(0xffffffffu, theirs_e);
+          if (in_place) cluster.sync();                 // every slot of the group has been read
+        } else {
+          const uint32_t total = __reduce_add_sync(0xffffffffu, count);
+          certain0 += static_cast<int>(total & 0xFFFFu);
+          equal0 += static_cast<int>(total >> 16);
+          if (in_place) __syncthreads();
+        }
+        if ((mine[g] >> 16) == 0u) {                    // no key of the warp equals the threshold
+          const int equals = min(equal, need);
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const bool stay = key[g][k] > threshold;
+            const unsigned stays = __ballot_sync(0xffffffffu, stay);
+            const int to = certain + equals + __popc(stays & before);
+            certain += __popc(stays);
+            if (stay) slots_out[to] = slot[k];
+            if (stay) weights_out[to] = w[k];
+            if (!stay && key[g][k] != kNothing) freed[at + k * 32 - to] = slot[k];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const bool sure = key[g][k] > threshold, same = key[g][k] == threshold;
+            const unsigned sures = __ballot_sync(0xffffffffu, sure), sames = __ballot_sync(0xffffffffu, same);
+            const int rank_same = equal + __popc(sames & before);
+            const int to = certain + __popc(sures & before) + min(rank_same, need);
+            const bool stay = sure || (same && rank_same < need);
+            certain += __popc(sures);
+            equal += __popc(sames);
+            if (stay) slots_out[to] = slot[k];
+            if (stay) weights_out[to] = w[k];
+            if (!stay && key[g][k] != kNothing) freed[at + k * 32 - to] = slot[k];
+          }
+        }
+      }
+    if (!once) __syncthreads();                         // counts are used again
   }
+  const int stays = idle ? n : certain0 + min(equal0, need);
+  for (int i = stays + rank * kThreads + tid; i < n; i += ctas * kThreads) weights_out[i] = 0.f;
+  if (ctas > 1) cluster.sync();                         // nobody reads this CTA's shared memory, or the length, any more
+  else __syncthreads();
+  if (rank == 0 && tid == 0) {
+    if (c.lens_dtype == AKL_IDX_I64) static_cast<long long*>(c.kv_lens_out)[b] = stays;
+    else static_cast<int*>(c.kv_lens_out)[b] = stays;
+    c.freed_lens[b] = n - stays;
+  }
+}
+
+template <typename Slot>
+int launch_evict(const akl_evict_t& c, int ctas, cudaStream_t s) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, evict_kernel<Slot>, c);
+  if (e != cudaSuccess) { note_cuda_error(e, "evict_kernel"); return AKL_ERR_CUDA; }
+  return AKL_OK;
 }
 
 }  // namespace
@@ -134,11 +358,17 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
   if (c->table_stride < c->table_width || c->table_out_stride < c->table_width || c->weights_stride < c->table_width ||
       c->weights_out_stride < c->table_width || c->freed_stride < c->freed_width)
     return AKL_ERR_INVALID;
+  if (c->table_width >= (1 << 30)) return AKL_ERR_UNSUPPORTED;      // positions are 32-bit, and rounds run past the end
   if (c->freed_width < c->table_width - c->keep) return AKL_ERR_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c->idx_dtype == AKL_IDX_I64) evict_kernel<long long><<<c->batch, kThreads, 0, s>>>(*c);
-  else evict_kernel<int><<<c->batch, kThreads, 0, s>>>(*c);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) { note_cuda_error(e, "evict_kernel"); return AKL_ERR_CUDA; }
-  return AKL_OK;
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != AKL_OK) return rc;
+  // Clusters while the requests leave SMs idle, but at least two steps for every thread of the widest row.
+  // (256 requests of up to 32768: 55 us with a CTA each, 71 with two, 108 with four; one of 139264: 177, 102, 58,
+  // 30 and 24 us with 1, 2, 4, 8 and 16.)
+  int ctas = 1;
+  while (ctas < kMaxCluster && static_cast<int64_t>(c->batch) * ctas * 2 <= sms && c->table_width > 2 * kThreads * ctas) ctas *= 2;
+  if (static_cast<int64_t>(c->batch) * ctas >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
+  return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, ctas, s) : launch_evict<int>(*c, ctas, s);
 }

@@ -168,6 +168,9 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
     _need("weights", weights, (torch.float32,), 2, device, "[rows, >= width]")
     _check_table("weights", weights)
     width = page_table.shape[1]
+    if width >= 1 << 30:
+        _reject(f"page_table rows of {width} entries: at most 2^30 - 1", field="page_table", value=width,
+                supported="< 2^30")
     if weights.shape[0] != page_table.shape[0] or weights.shape[1] < width:
         _reject(f"weights shape {tuple(weights.shape)} must cover the page table's {tuple(page_table.shape)}",
                 field="weights", value=tuple(weights.shape), supported=tuple(page_table.shape))
