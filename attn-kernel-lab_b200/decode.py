@@ -16,8 +16,9 @@ import math
 
 import torch
 
+from . import kernel
 from .capability import DECODE_CAPABILITY, CapabilityError, OperatorCapability, check_supported
-from .ops import _dtype_name, _reject, _same_device, _shares_storage
+from .ops import _dtype_name, _reject, _same_device
 
 __all__ = ["DecodeWorkspace", "check_decode", "paged_decode", "plan_decode_workspace"]
 
@@ -40,6 +41,7 @@ class _Scratch:
         at = self._ptr - self._buf.data_ptr() + int(layout.off_status)
         self._status = self._buf[at:at + 256].view(torch.int32)
         self._status.zero_()
+        self.device_index = -1 if self.device.type != "cuda" else self.device.index
 
     def base_ptr(self) -> int:
         return self._ptr
@@ -69,8 +71,6 @@ class DecodeWorkspace(_Scratch):
     lengths, each rounded up to 64.  0 reserves nothing for weights."""
 
     def __init__(self, device, *, max_requests: int, q_heads: int, kv_heads: int, max_weight_tokens: int = 0):
-        from . import kernel
-
         _check_sizes(max_requests=max_requests, q_heads=q_heads, kv_heads=kv_heads,
                      max_weight_tokens=max_weight_tokens)
         self.plan = kernel.DecodePlan(max_requests, q_heads, kv_heads, 0, max_weight_tokens)
@@ -78,6 +78,17 @@ class DecodeWorkspace(_Scratch):
         kernel.check(kernel.load().akl_decode_layout(ctypes.byref(self.plan), ctypes.byref(layout)),
                      "akl_decode_layout")
         super().__init__(device, layout)
+        self._plan_fields = (max_requests, q_heads, kv_heads, 0, max_weight_tokens)
+        self._declared = _declares(q_heads, kv_heads, "decode")
+
+
+def _declares(q_heads: int, kv_heads: int, mode: str) -> bool:
+    """Whether the default surface has these heads."""
+    try:
+        _check_heads(q_heads, kv_heads, 256, "bfloat16", mode, False, DECODE_CAPABILITY)
+    except CapabilityError:
+        return False
+    return True
 
 
 def _check_heads(q_heads: int, kv_heads: int, head_dim: int, kv_dtype: str, mode: str, return_lse: bool,
@@ -142,6 +153,19 @@ def _check_decay(weight_decay) -> None:
     if isinstance(weight_decay, bool) or not isinstance(weight_decay, (int, float)) or not 0.0 <= weight_decay <= 1.0:
         _reject(f"weight_decay must be a number in [0, 1], got {weight_decay!r}", field="weight_decay",
                 value=weight_decay, supported="[0, 1]")
+
+
+def _overlap(a, b) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    if a.device.type == "meta" or b.device.type == "meta":
+        return False
+
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 def _row_stride(t) -> int:
@@ -218,8 +242,8 @@ def check_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
                     f"{tuple(out.stride())}", field="out", value=tuple(out.shape), supported=tuple(q.shape))
         if out.data_ptr() & 15:
             _reject("out must start on a 16-byte boundary", field="out", value=out.data_ptr() & 15, supported=0)
-        if _shares_storage(out, q):
-            _reject("out must not overlap q storage", field="out", value="aliases q", supported="a distinct allocation")
+        if _overlap(out, q):
+            _reject("out must not overlap q", field="out", value="aliases q", supported="memory of its own")
     if lse_out is not None:
         if not return_lse:
             _reject("lse_out was supplied but return_lse=False: a destination for an output that will not be "
@@ -256,16 +280,16 @@ def _admit(ws: DecodeWorkspace, batch: int, q_heads: int, kv_heads: int, weights
             f"max_weight_tokens={p.max_weight_tokens}); the allocation never changes")
 
 
-def _call(device, fn, name, struct) -> None:
-    """One native call on the tensors' device and its current stream."""
-    from . import kernel
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index is None or device.index == torch.cuda.current_device():
-        code = fn(ctypes.byref(struct), stream)
+
+def _call(index: int, fn, name: str, packed: bytes) -> None:
+    """One native call on CUDA device `index` and its current stream."""
+    if index == torch.cuda.current_device():
+        code = fn(packed, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            code = fn(ctypes.byref(struct), stream)
+        with torch.cuda.device(index):
+            code = fn(packed, _raw_stream(index))
     if code:
         kernel.check(code, name)
 
@@ -298,13 +322,19 @@ def paged_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
     the weights of the last requests are not).
 
     Returns `out` [batch, q_heads, 256] BF16, or `(out, lse)` with the base-2 `lse` [batch, q_heads]."""
+    if workspace is not None and out is not None and capability is DECODE_CAPABILITY:
+        packed = _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, workspace, out, lse_out, weights, weight_decay,
+                           sm_scale, return_lse)
+        if packed is not None:
+            _call(workspace.device_index, kernel.load().akl_paged_decode, "akl_paged_decode", packed)
+            if check_status:
+                _raise_on_status(workspace, "akl_paged_decode")
+            return (out, lse_out) if return_lse else out
     batch, q_heads, kv_heads = check_decode(
         q, k_pool, v_pool, page_table, kv_lens, rows=rows, workspace=workspace, out=out, lse_out=lse_out,
         weights=weights, weight_decay=weight_decay, sm_scale=sm_scale, return_lse=return_lse, capability=capability)
     device = q.device
     _need_cuda("paged_decode", device)
-    from . import kernel
-
     lib = kernel.load()
     table_rows, width = page_table.shape
     if workspace is None:
@@ -316,20 +346,86 @@ def paged_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
         out = torch.empty((batch, q_heads, 256), dtype=torch.bfloat16, device=device)
     if return_lse and lse_out is None:
         lse_out = torch.empty((batch, q_heads), dtype=torch.float32, device=device)
-    call = kernel.Decode(
+    packed = kernel.pack_decode(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(),
-        None if rows is None else rows.data_ptr(), kv_lens.data_ptr(), out.data_ptr(),
-        lse_out.data_ptr() if return_lse else None, None if weights is None else weights.data_ptr(),
-        workspace._ptr, workspace._bytes, workspace.plan, k_pool.shape[0],
+        0 if rows is None else rows.data_ptr(), kv_lens.data_ptr(), out.data_ptr(),
+        lse_out.data_ptr() if return_lse else 0, 0 if weights is None else weights.data_ptr(),
+        workspace._ptr, workspace._bytes, *workspace._plan_fields, k_pool.shape[0],
         q.stride(0) if batch > 1 else q_heads * 256, _pool_stride(k_pool), _pool_stride(v_pool),
         _row_stride(page_table), 0 if weights is None else _row_stride(weights),
         batch, q_heads, kv_heads, table_rows, width, _KV[k_pool.dtype], _INDEX[page_table.dtype],
         0 if rows is None else _INDEX[rows.dtype], _INDEX[kv_lens.dtype],
-        1.0 / 16.0 if sm_scale is None else sm_scale, weight_decay)
-    _call(device, lib.akl_paged_decode, "akl_paged_decode", call)
+        0.0625 if sm_scale is None else sm_scale, 1.0 if weights is None else weight_decay)
+    _call(workspace.device_index, lib.akl_paged_decode, "akl_paged_decode", packed)
     if check_status:
         _raise_on_status(workspace, "akl_paged_decode")
     return (out, lse_out) if return_lse else out
+
+
+def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, weights, weight_decay, sm_scale,
+              return_lse):
+    """The packed call when every argument has its ordinary form -- contiguous tensors of the expected
+    types on one GPU, a plan that admits them -- or None: `check_decode` then looks closer, and either
+    accepts or says what is wrong.  A single step is short enough for the checks to show (they were 15
+    of 26 us a call), and these few comparisons are the same ones."""
+    try:
+        if type(ws) is not DecodeWorkspace or not ws._declared:
+            return None
+        index = ws.device_index
+        max_requests, q_heads, kv_heads, _, max_tokens = ws._plan_fields
+        batch, heads, dim = q.shape
+        pool_shape = k_pool.shape
+        pool, kv, kv_dim = pool_shape
+        table_shape = page_table.shape
+        table_rows, width = table_shape
+        kv_type, idx_type, lens_type = _KV[k_pool.dtype], _INDEX[page_table.dtype], _INDEX[kv_lens.dtype]
+        if (index < 0 or heads != q_heads or kv != kv_heads or dim != 256 or kv_dim != 256
+                or not 1 <= batch <= max_requests or not 1 <= pool < 1 << 31 or not 1 <= table_rows < 1 << 31
+                or not 1 <= width < 1 << 31 or v_pool.shape != pool_shape or v_pool.dtype is not k_pool.dtype
+                or q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q.shape
+                or kv_lens.shape != (batch,)
+                or not (q.is_contiguous() and k_pool.is_contiguous() and v_pool.is_contiguous()
+                        and page_table.is_contiguous() and kv_lens.is_contiguous() and out.is_contiguous())
+                or not (q.get_device() == k_pool.get_device() == v_pool.get_device() == page_table.get_device()
+                        == kv_lens.get_device() == out.get_device() == index)):
+            return None
+        rows_ptr = rows_type = lse_ptr = weights_ptr = 0
+        if rows is not None:
+            rows_type = _INDEX[rows.dtype]
+            if rows.shape != (batch,) or not rows.is_contiguous() or rows.get_device() != index:
+                return None
+            rows_ptr = rows.data_ptr()
+        elif table_rows < batch:
+            return None
+        if return_lse:
+            if (lse_out.dtype is not torch.float32 or lse_out.shape != (batch, heads) or not lse_out.is_contiguous()
+                    or lse_out.get_device() != index):
+                return None
+            lse_ptr = lse_out.data_ptr()
+        elif lse_out is not None:
+            return None
+        if weights is None:
+            weight_decay = 1.0
+        else:
+            if (not max_tokens or weights.dtype is not torch.float32 or weights.shape != table_shape
+                    or not weights.is_contiguous() or weights.get_device() != index
+                    or type(weight_decay) is not float or not 0.0 <= weight_decay <= 1.0):
+                return None
+            weights_ptr = weights.data_ptr()
+        if sm_scale is None:
+            sm_scale = 0.0625
+        elif type(sm_scale) is not float or not 0.0 < sm_scale < math.inf:
+            return None
+        q_ptr, k_ptr, v_ptr, out_ptr = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+        row = heads * 256
+        if (q_ptr | k_ptr | v_ptr | out_ptr) & 15 or abs(out_ptr - q_ptr) < batch * row * 2:
+            return None
+    except (AttributeError, TypeError, ValueError, KeyError):
+        return None
+    return kernel.pack_decode(
+        q_ptr, k_ptr, v_ptr, page_table.data_ptr(), rows_ptr, kv_lens.data_ptr(), out_ptr, lse_ptr, weights_ptr, ws._ptr,
+        ws._bytes, *ws._plan_fields, pool, row, kv * 256, kv * 256, width, width if weights_ptr else 0, batch, heads, kv, table_rows, width,
+        kv_type, idx_type, rows_type, lens_type, sm_scale, weight_decay)
 
 
 def _pool_stride(t) -> int:
@@ -337,7 +433,6 @@ def _pool_stride(t) -> int:
 
 
 def _raise_on_status(ws, where: str) -> None:
-    from . import kernel
     from .ops import _raise_on_status as raise_on_status
 
     raise_on_status(ws, kernel, where)

@@ -11,14 +11,16 @@ The reference has no counterpart; validation, errors, workspaces and streams are
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
+from . import kernel
 from .capability import DECODE_CAPABILITY, OperatorCapability
 from .decode import (_INDEX, _KV, _Scratch, _call, _check_batch_vector, _check_decay, _check_heads, _check_rows,
-                     _check_scale, _check_sizes, _check_table, _need, _need_cuda, _pool_stride, _raise_on_status,
-                     _row_stride)
-from .ops import _dtype_name, _reject, _same_device, _shares_storage
+                     _check_scale, _check_sizes, _check_table, _declares, _need, _need_cuda, _overlap, _pool_stride,
+                     _raise_on_status, _row_stride)
+from .ops import _dtype_name, _reject, _same_device
 
 __all__ = ["WeightsWorkspace", "evict_lightest", "extend_weights", "plan_weights_workspace"]
 
@@ -27,14 +29,14 @@ class WeightsWorkspace(_Scratch):
     """Capacity-reserved scratch of `extend_weights`; one call at a time (stream order) may use it."""
 
     def __init__(self, device, *, max_kv_len: int, max_q_len: int, q_heads: int, kv_heads: int):
-        from . import kernel
-
         _check_sizes(max_kv_len=max_kv_len, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
         self.plan = kernel.WeightsPlan(max_kv_len, max_q_len, q_heads, kv_heads)
         layout = kernel.WeightsLayout()
         kernel.check(kernel.load().akl_weights_layout(ctypes.byref(self.plan), ctypes.byref(layout)),
                      "akl_weights_layout")
         super().__init__(device, layout)
+        self._plan_fields = (max_kv_len, max_q_len, q_heads, kv_heads)
+        self._declared = _declares(q_heads, kv_heads, "extend_weights")
 
 
 def plan_weights_workspace(device, *, max_kv_len: int, max_q_len: int, q_heads: int | None = None,
@@ -84,9 +86,8 @@ def _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace,
     if weights.shape[0] != kv_len or not weights.is_contiguous():
         _reject(f"weights must be contiguous [{kv_len}], got {tuple(weights.shape)} with stride {weights.stride()}",
                 field="weights", value=tuple(weights.shape), supported=(kv_len,))
-    if _shares_storage(weights, lse):
-        _reject("weights must not overlap lse storage", field="weights", value="aliases lse",
-                supported="a distinct allocation")
+    if _overlap(weights, lse):
+        _reject("weights must not overlap lse", field="weights", value="aliases lse", supported="memory of its own")
     _check_decay(weight_decay)
     if sm_scale is not None:
         _check_scale(sm_scale)
@@ -116,11 +117,16 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
 
     Enqueues on the current stream and does not synchronise unless `check_status` (a debugging aid).
     Returns `weights`."""
+    if workspace is not None and capability is DECODE_CAPABILITY:
+        packed = _ordinary_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale)
+        if packed is not None:
+            _call(workspace.device_index, kernel.load().akl_extend_weights, "akl_extend_weights", packed)
+            if check_status:
+                _raise_on_status(workspace, "akl_extend_weights")
+            return weights
     _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale, capability)
     device = q.device
     _need_cuda("extend_weights", device)
-    from . import kernel
-
     lib = kernel.load()
     q_len, q_heads = q.shape[:2]
     kv_heads, kv_len = k_pool.shape[1], idx.shape[0]
@@ -135,15 +141,50 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
                 f"extend of {q_len} rows over {kv_len} positions at {q_heads}:{kv_heads} heads is outside the "
                 f"workspace plan (max_q_len={p.max_q_len}, max_kv_len={p.max_kv_len}, heads "
                 f"{p.q_heads}:{p.kv_heads}); the allocation never changes")
-    call = kernel.Weights(
+    packed = kernel.pack_weights(
         q.data_ptr(), k_pool.data_ptr(), idx.data_ptr(), lse.data_ptr(), weights.data_ptr(), workspace._ptr,
-        workspace._bytes, workspace.plan, k_pool.shape[0], q.stride(0) if q_len > 1 else q_heads * 256,
+        workspace._bytes, *workspace._plan_fields, k_pool.shape[0], q.stride(0) if q_len > 1 else q_heads * 256,
         _pool_stride(k_pool), q_len, kv_len, prefix, q_heads, kv_heads, _KV[k_pool.dtype], _INDEX[idx.dtype],
-        1.0 / 16.0 if sm_scale is None else sm_scale, weight_decay)
-    _call(device, lib.akl_extend_weights, "akl_extend_weights", call)
+        0.0625 if sm_scale is None else sm_scale, weight_decay)
+    _call(workspace.device_index, lib.akl_extend_weights, "akl_extend_weights", packed)
     if check_status:
         _raise_on_status(workspace, "akl_extend_weights")
     return weights
+
+
+def _ordinary_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, ws, sm_scale):
+    """The packed call when every argument has its ordinary form, or None: the full checks then decide
+    (as `decode._ordinary`)."""
+    try:
+        if type(ws) is not WeightsWorkspace or not ws._declared:
+            return None
+        index = ws.device_index
+        max_kv_len, max_q_len, q_heads, kv_heads = ws._plan_fields
+        q_len, heads, dim = q.shape
+        pool, kv, kv_dim = k_pool.shape
+        kv_len, = idx.shape
+        kv_type, idx_type = _KV[k_pool.dtype], _INDEX[idx.dtype]
+        if sm_scale is None:
+            sm_scale = 0.0625
+        if (index < 0 or heads != q_heads or kv != kv_heads or dim != 256 or kv_dim != 256 or not 1 <= q_len <= max_q_len
+                or not 1 <= kv_len <= max_kv_len or pool < 1 or type(prefix) is not int or not 0 <= prefix <= kv_len - q_len
+                or q.dtype is not torch.bfloat16 or lse.dtype is not torch.float32 or lse.shape != (q_len, heads)
+                or weights.dtype is not torch.float32 or weights.shape != (kv_len,)
+                or type(sm_scale) is not float or not 0.0 < sm_scale < math.inf
+                or type(weight_decay) is not float or not 0.0 <= weight_decay <= 1.0
+                or not (q.is_contiguous() and k_pool.is_contiguous() and idx.is_contiguous() and lse.is_contiguous()
+                        and weights.is_contiguous())
+                or not (q.get_device() == k_pool.get_device() == idx.get_device() == lse.get_device()
+                        == weights.get_device() == index)):
+            return None
+        q_ptr, k_ptr, lse_ptr, weights_ptr = q.data_ptr(), k_pool.data_ptr(), lse.data_ptr(), weights.data_ptr()
+        if (q_ptr | k_ptr) & 15 or (weights_ptr < lse_ptr + q_len * heads * 4 and lse_ptr < weights_ptr + kv_len * 4):
+            return None
+    except (AttributeError, TypeError, ValueError, KeyError):
+        return None
+    return kernel.pack_weights(q_ptr, k_ptr, idx.data_ptr(), lse_ptr, weights_ptr, ws._ptr, ws._bytes, *ws._plan_fields,
+                               pool, heads * 256, kv * 256, q_len, kv_len, prefix, heads, kv, kv_type, idx_type, sm_scale,
+                               weight_decay)
 
 
 def _check_out(name, t, like, source_name) -> None:
@@ -155,7 +196,7 @@ def _check_out(name, t, like, source_name) -> None:
         _reject(f"{name} shape {tuple(t.shape)} must equal {source_name}'s {tuple(like.shape)}", field=name,
                 value=tuple(t.shape), supported=tuple(like.shape))
     _check_table(name, t)
-    if _shares_storage(t, like) and (t.data_ptr() != like.data_ptr() or _row_stride(t) != _row_stride(like)):
+    if _overlap(t, like) and (t.data_ptr() != like.data_ptr() or _row_stride(t) != _row_stride(like)):
         _reject(f"{name} overlaps {source_name} at another address: it must be {source_name} itself or a distinct "
                 "allocation", field=name, value="overlaps", supported=f"{source_name} or a distinct allocation")
 
@@ -198,7 +239,7 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
             _reject(f"kv_lens_out dtype {_dtype_name(lens_out.dtype)} must equal kv_lens dtype "
                     f"{_dtype_name(kv_lens.dtype)}", field="kv_lens_out", value=_dtype_name(lens_out.dtype),
                     supported=_dtype_name(kv_lens.dtype))
-        if _shares_storage(lens_out, kv_lens) and lens_out.data_ptr() != kv_lens.data_ptr():
+        if _overlap(lens_out, kv_lens) and lens_out.data_ptr() != kv_lens.data_ptr():
             _reject("kv_lens_out overlaps kv_lens at another address", field="kv_lens_out", value="overlaps",
                     supported="kv_lens or a distinct allocation")
     if freed is not None:
@@ -207,13 +248,13 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
             _reject(f"freed shape {tuple(freed.shape)} must be at least {(batch, max(1, width - keep))}", field="freed",
                     value=tuple(freed.shape), supported=(batch, max(1, width - keep)))
         _check_table("freed", freed)
-        if _shares_storage(freed, page_table) or _shares_storage(freed, table_out):
+        if _overlap(freed, page_table) or _overlap(freed, table_out):
             _reject("freed must not overlap the page table", field="freed", value="overlaps",
                     supported="a distinct allocation")
     if freed_lens is not None:
         _need("freed_lens", freed_lens, (torch.int32,), 1, device, "[batch]")
         _check_batch_vector("freed_lens", freed_lens, batch, device)
-        if _shares_storage(freed_lens, kv_lens) or _shares_storage(freed_lens, lens_out):
+        if _overlap(freed_lens, kv_lens) or _overlap(freed_lens, lens_out):
             _reject("freed_lens must not overlap kv_lens", field="freed_lens", value="overlaps",
                     supported="a distinct allocation")
 
@@ -239,23 +280,90 @@ def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: in
     table_out = page_table if page_table_out is None else page_table_out
     acc_out = weights if weights_out is None else weights_out
     lens_out = kv_lens if kv_lens_out is None else kv_lens_out
-    _check_evict(page_table, weights, kv_lens, keep, protect_first, protect_last, rows, table_out, acc_out, lens_out,
-                 freed, freed_lens)
-    device = page_table.device
-    _need_cuda("evict_lightest", device)
-    from . import kernel
-
-    lib = kernel.load()
-    batch, (table_rows, width) = kv_lens.shape[0], page_table.shape
-    if freed is None:
-        freed = torch.empty((batch, max(1, width - keep)), dtype=page_table.dtype, device=device)
-    if freed_lens is None:
-        freed_lens = torch.empty(batch, dtype=torch.int32, device=device)
-    call = kernel.Evict(
-        page_table.data_ptr(), weights.data_ptr(), None if rows is None else rows.data_ptr(), kv_lens.data_ptr(),
-        table_out.data_ptr(), acc_out.data_ptr(), lens_out.data_ptr(), freed.data_ptr(), freed_lens.data_ptr(),
-        _row_stride(page_table), _row_stride(weights), _row_stride(table_out), _row_stride(acc_out), _row_stride(freed),
-        batch, table_rows, width, freed.shape[1], keep, protect_first, protect_last, _INDEX[page_table.dtype],
-        0 if rows is None else _INDEX[rows.dtype], _INDEX[kv_lens.dtype])
-    _call(device, lib.akl_evict_lightest, "akl_evict_lightest", call)
+    index, packed = _ordinary_evict(page_table, weights, kv_lens, keep, protect_first, protect_last, rows, table_out,
+                                    acc_out, lens_out, freed, freed_lens)
+    if packed is None:
+        _check_evict(page_table, weights, kv_lens, keep, protect_first, protect_last, rows, table_out, acc_out, lens_out,
+                     freed, freed_lens)
+        device = page_table.device
+        _need_cuda("evict_lightest", device)
+        index = device.index if device.index is not None else torch.cuda.current_device()
+        batch, (table_rows, width) = kv_lens.shape[0], page_table.shape
+        if freed is None:
+            freed = torch.empty((batch, max(1, width - keep)), dtype=page_table.dtype, device=device)
+        if freed_lens is None:
+            freed_lens = torch.empty(batch, dtype=torch.int32, device=device)
+        packed = kernel.pack_evict(
+            page_table.data_ptr(), weights.data_ptr(), 0 if rows is None else rows.data_ptr(), kv_lens.data_ptr(),
+            table_out.data_ptr(), acc_out.data_ptr(), lens_out.data_ptr(), freed.data_ptr(), freed_lens.data_ptr(),
+            _row_stride(page_table), _row_stride(weights), _row_stride(table_out), _row_stride(acc_out),
+            _row_stride(freed), batch, table_rows, width, freed.shape[1], keep, protect_first, protect_last,
+            _INDEX[page_table.dtype], 0 if rows is None else _INDEX[rows.dtype], _INDEX[kv_lens.dtype])
+    _call(index, kernel.load().akl_evict_lightest, "akl_evict_lightest", packed)
     return table_out, acc_out, lens_out, freed, freed_lens
+
+
+def _ordinary_evict(page_table, weights, kv_lens, keep, first, last, rows, table_out, acc_out, lens_out, freed,
+                    freed_lens):
+    """(device index, packed call) when every argument has its ordinary form, or (None, None): the full checks
+    then decide (as `decode._ordinary`)."""
+    no = None, None
+    try:
+        index = page_table.get_device()
+        shape = page_table.shape
+        table_rows, width = shape
+        batch, = kv_lens.shape
+        idx_type, lens_type = _INDEX[page_table.dtype], _INDEX[kv_lens.dtype]
+        freed_rows, freed_width = freed.shape
+        if (index < 0 or table_rows < 1 or not 1 <= width < 1 << 30 or table_rows >= 1 << 31 or batch < 1
+                or weights.shape != shape or weights.dtype is not torch.float32
+                or type(keep) is not int or type(first) is not int or type(last) is not int
+                or first < 0 or last < 0 or not max(1, first + last) <= keep < 1 << 31
+                or freed_rows != batch or freed_width < max(1, width - keep) or freed.dtype is not page_table.dtype
+                or freed_lens.shape != (batch,) or freed_lens.dtype is not torch.int32
+                or not (page_table.is_contiguous() and weights.is_contiguous() and kv_lens.is_contiguous()
+                        and freed.is_contiguous() and freed_lens.is_contiguous())
+                or not (weights.get_device() == kv_lens.get_device() == freed.get_device() == freed_lens.get_device()
+                        == index)):
+            return no
+        table_ptr, weights_ptr, lens_ptr = page_table.data_ptr(), weights.data_ptr(), kv_lens.data_ptr()
+        freed_ptr, count_ptr = freed.data_ptr(), freed_lens.data_ptr()
+        table_out_ptr, acc_out_ptr, lens_out_ptr = table_ptr, weights_ptr, lens_ptr
+        item = 8 if idx_type == 0 else 4
+        table_bytes, acc_bytes = table_rows * width * item, table_rows * width * 4
+        lens_bytes = batch * (8 if lens_type == 0 else 4)
+        for out, src in ((table_out, page_table), (acc_out, weights), (lens_out, kv_lens)):
+            if out is not src and (out.dtype is not src.dtype or out.shape != src.shape or not out.is_contiguous()
+                                   or out.get_device() != index):
+                return no
+        if table_out is not page_table:
+            table_out_ptr = table_out.data_ptr()
+            if 0 < abs(table_out_ptr - table_ptr) < table_bytes:
+                return no
+        if acc_out is not weights:
+            acc_out_ptr = acc_out.data_ptr()
+            if 0 < abs(acc_out_ptr - weights_ptr) < acc_bytes:
+                return no
+        if lens_out is not kv_lens:
+            lens_out_ptr = lens_out.data_ptr()
+            if 0 < abs(lens_out_ptr - lens_ptr) < lens_bytes:
+                return no
+        for at in (table_ptr, table_out_ptr):
+            if freed_ptr < at + table_bytes and at < freed_ptr + batch * freed_width * item:
+                return no
+        for at in (lens_ptr, lens_out_ptr):
+            if count_ptr < at + lens_bytes and at < count_ptr + batch * 4:
+                return no
+        rows_ptr = rows_type = 0
+        if rows is not None:
+            rows_type = _INDEX[rows.dtype]
+            if rows.shape != (batch,) or not rows.is_contiguous() or rows.get_device() != index:
+                return no
+            rows_ptr = rows.data_ptr()
+        elif table_rows < batch:
+            return no
+    except (AttributeError, TypeError, ValueError, KeyError):
+        return no
+    return index, kernel.pack_evict(table_ptr, weights_ptr, rows_ptr, lens_ptr, table_out_ptr, acc_out_ptr, lens_out_ptr,
+                                    freed_ptr, count_ptr, width, width, width, width, freed_width, batch, table_rows, width,
+                                    freed_width, keep, first, last, idx_type, rows_type, lens_type)

@@ -34,7 +34,7 @@ def test_decode_accepts_the_geometry_then_needs_a_gpu(pkg):
         pkg.paged_decode(**_decode())
 
 
-@pytest.mark.parametrize("field,over", [
+DECODE_REFUSALS = [
     ("q", dict(q=None)), ("q", dict(q=torch.zeros(2, 24 * 256, dtype=torch.bfloat16))),
     ("q", dict(q=torch.zeros(2, 24, 256))), ("q", dict(q=torch.zeros(0, 24, 256, dtype=torch.bfloat16))),
     ("q", dict(q=torch.zeros(24, 2, 256, dtype=torch.bfloat16).transpose(0, 1))),
@@ -62,7 +62,11 @@ def test_decode_accepts_the_geometry_then_needs_a_gpu(pkg):
     ("weight_decay", dict(weights=torch.zeros(4, 12), weight_decay=float("nan"))),
     ("workspace", dict(workspace=object())),
     ("kv_lens", dict(kv_lens=torch.zeros(2, dtype=torch.int32, device="meta"))),
-], ids=lambda v: v if isinstance(v, str) else ",".join(v))
+]
+_IDS = lambda v: v if isinstance(v, str) else ",".join(v)      # noqa: E731
+
+
+@pytest.mark.parametrize("field,over", DECODE_REFUSALS, ids=_IDS)
 def test_decode_refusals(pkg, field, over):
     _refused(pkg, field, **over)
 
@@ -90,7 +94,7 @@ def _extend(**over):
     return kw
 
 
-@pytest.mark.parametrize("field,over", [
+EXTEND_REFUSALS = [
     ("q", dict(q=torch.zeros(4, 24, 256))), ("q_len", dict(q=torch.zeros(0, 24, 256, dtype=torch.bfloat16))),
     ("kv_heads", dict(k_pool=torch.zeros(40, 6, 256, dtype=torch.float16))),
     ("idx", dict(idx=torch.zeros(0, dtype=torch.int64))), ("idx", dict(idx=torch.zeros(20))),
@@ -98,7 +102,10 @@ def _extend(**over):
     ("lse", dict(lse=torch.zeros(24, 4).T)), ("lse", dict(lse=torch.zeros(4, 24, dtype=torch.float64))),
     ("weights", dict(weights=torch.zeros(21))), ("weights", dict(weights=torch.zeros(40)[::2])),
     ("weight_decay", dict(weight_decay=-0.5)), ("sm_scale", dict(sm_scale=-1.0)), ("workspace", dict(workspace=3)),
-], ids=lambda v: v if isinstance(v, str) else ",".join(v))
+]
+
+
+@pytest.mark.parametrize("field,over", EXTEND_REFUSALS, ids=_IDS)
 def test_extend_weights_refusals(pkg, field, over):
     with pytest.raises(pkg.CapabilityError) as e:
         pkg.extend_weights(**_extend(**over))
@@ -120,7 +127,7 @@ def _evict(**over):
 _TABLE = torch.zeros(5, 12, dtype=torch.int32)
 
 
-@pytest.mark.parametrize("field,over", [
+EVICT_REFUSALS = [
     ("page_table", dict(page_table=torch.zeros(4, 12))), ("weights", dict(weights=torch.zeros(4, 11))),
     ("weights", dict(weights=torch.zeros(3, 12))), ("kv_lens", dict(kv_lens=torch.zeros(0, dtype=torch.int64))),
     ("page_table", dict(kv_lens=torch.zeros(5, dtype=torch.int64))), ("rows", dict(rows=torch.zeros(3, dtype=torch.int32))),
@@ -133,7 +140,10 @@ _TABLE = torch.zeros(5, 12, dtype=torch.int32)
     ("kv_lens_out", dict(kv_lens_out=torch.zeros(2, dtype=torch.int32))),
     ("freed", dict(freed=torch.zeros(2, 3, dtype=torch.int32))), ("freed", dict(freed=torch.zeros(2, 4, dtype=torch.int64))),
     ("freed_lens", dict(freed_lens=torch.zeros(2, dtype=torch.int64))),
-], ids=lambda v: v if isinstance(v, str) else ",".join(v))
+]
+
+
+@pytest.mark.parametrize("field,over", EVICT_REFUSALS, ids=_IDS)
 def test_eviction_refusals(pkg, field, over):
     with pytest.raises(pkg.CapabilityError) as e:
         pkg.evict_lightest(**_evict(**over))
@@ -143,6 +153,99 @@ def test_eviction_refusals(pkg, field, over):
 def test_eviction_needs_a_gpu(pkg):
     with pytest.raises(RuntimeError, match="no CPU path"):
         pkg.evict_lightest(**_evict())
+
+
+# ---- the short form of the checks: what it takes it packs as the full form does, the rest it leaves alone
+@pytest.fixture()
+def short(pkg, monkeypatch):
+    """CPU tensors stand for those of GPU 0 (nothing is launched); calls are recorded, not made."""
+    from attn_kernel_lab_b200 import decode, eviction
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(decode, "_need_cuda", lambda *a: None)
+    monkeypatch.setattr(eviction, "_need_cuda", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    seen = []
+    for module in (decode, eviction):
+        monkeypatch.setattr(module, "_call", lambda index, fn, name, packed: seen.append((index, name, packed)))
+    return decode, eviction, seen
+
+
+def _on_gpu0(ws):
+    ws.device_index = 0
+    return ws
+
+
+@pytest.mark.parametrize("rows", [True, False])
+@pytest.mark.parametrize("weights", [None, 0.5])
+@pytest.mark.parametrize("lse", [True, False])
+def test_short_decode_packs_what_the_full_form_packs(pkg, short, monkeypatch, rows, weights, lse):
+    decode, _, seen = short
+    ws = _on_gpu0(pkg.plan_decode_workspace("cpu", max_requests=3, q_heads=24, kv_heads=4, max_weight_tokens=640))
+    kw = _decode(workspace=ws, out=torch.zeros(2, 24, 256, dtype=torch.bfloat16), sm_scale=0.125)
+    if not rows:
+        kw["rows"] = None
+    if weights is not None:
+        kw.update(weights=torch.zeros(kw["page_table"].shape), weight_decay=weights)
+    if lse:
+        kw.update(return_lse=True, lse_out=torch.zeros(2, 24))
+    pkg.paged_decode(**kw)
+    monkeypatch.setattr(decode, "_ordinary", lambda *a: None)
+    pkg.paged_decode(**kw)
+    assert len(seen) == 2 and seen[0] == seen[1]
+
+
+@pytest.mark.parametrize("field,over", DECODE_REFUSALS, ids=_IDS)
+def test_short_decode_leaves_refusals_to_the_full_form(pkg, short, field, over):
+    decode, _, seen = short
+    kw = dict(return_lse=False)
+    kw.update(_decode(workspace=_on_gpu0(pkg.plan_decode_workspace("cpu", max_requests=3, q_heads=24, kv_heads=4,
+                                                                   max_weight_tokens=640)),
+                      out=torch.zeros(2, 24, 256, dtype=torch.bfloat16)))
+    kw.update(over)
+    if any(isinstance(v, torch.Tensor) and v.device.type == "meta" for v in over.values()):
+        pytest.skip("every tensor is on GPU 0 here")
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.paged_decode(**kw)
+    assert e.value.field == field and not seen
+
+
+def test_short_extend_and_eviction_pack_what_the_full_forms_pack(pkg, short, monkeypatch):
+    _, eviction, seen = short
+    ws = _on_gpu0(pkg.plan_weights_workspace("cpu", max_kv_len=64, max_q_len=8, q_heads=24, kv_heads=4))
+    kw = _extend(workspace=ws, weight_decay=0.25)
+    outs = dict(freed=torch.zeros(2, 6, dtype=torch.int32), freed_lens=torch.zeros(2, dtype=torch.int32))
+    ev = [dict(_evict(weights=torch.zeros(4, 12)), **outs),
+          dict(_evict(weights=torch.zeros(4, 12), rows=torch.zeros(2, dtype=torch.int32)), **outs,
+               page_table_out=torch.zeros(4, 12, dtype=torch.int32), weights_out=torch.zeros(4, 12),
+               kv_lens_out=torch.zeros(2, dtype=torch.int64))]
+    for _ in range(2):
+        pkg.extend_weights(**kw)
+        for e in ev:
+            pkg.evict_lightest(**e)
+        monkeypatch.setattr(eviction, "_ordinary_extend", lambda *a: None)
+        monkeypatch.setattr(eviction, "_ordinary_evict", lambda *a: (None, None))
+    # (the full form names the device of the tensors, which the stand-ins do not have)
+    assert [s[1:] for s in seen[:3]] == [s[1:] for s in seen[3:]] and len({s[2] for s in seen[:3]}) == 3
+
+
+@pytest.mark.parametrize("field,over", EXTEND_REFUSALS, ids=_IDS)
+def test_short_extend_leaves_refusals_to_the_full_form(pkg, short, field, over):
+    ws = _on_gpu0(pkg.plan_weights_workspace("cpu", max_kv_len=64, max_q_len=8, q_heads=24, kv_heads=4))
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.extend_weights(**dict(_extend(workspace=ws), **over))
+    assert e.value.field == field and not short[2]
+
+
+@pytest.mark.parametrize("field,over", EVICT_REFUSALS, ids=_IDS)
+def test_short_eviction_leaves_refusals_to_the_full_form(pkg, short, field, over):
+    base = dict(_evict(weights=torch.zeros(4, 12)), freed=torch.zeros(2, 6, dtype=torch.int32),
+                freed_lens=torch.zeros(2, dtype=torch.int32))
+    if field == "weights_out":
+        over = dict(weights_out=torch.zeros(4, 13))
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.evict_lightest(**dict(base, **over))
+    assert e.value.field == field and not short[2]
 
 
 # ---- C entry points: every case fails host validation, so no pointer is followed -----------------
