@@ -49,7 +49,6 @@ constexpr int kWarps = 8;           // consumers
 constexpr int kProducers = 4;       // and the warps that gather for them
 constexpr int kThreads = (kWarps + kProducers) * 32;
 constexpr int kAhead = 4;           // tiles whose page-table entries are on their way
-constexpr int kMinTiles = 1;        // tiles a CTA takes at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr long long kWaitCycles = 4000000000ll;      // ~2 s: a wait that long is a defect
 
@@ -393,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   }
   Cursor<HB> at(c, lane);
   const long long total = at.total();
-  long long ctas = (total + kMinTiles - 1) / kMinTiles;
-  if (ctas > gridDim.x) ctas = gridDim.x;
+  // (at least two tiles a CTA made one request of 1000 positions 10.1 us instead of 8.7, and nothing faster)
+  const long long ctas = min(total, static_cast<long long>(gridDim.x));
   if (blockIdx.x >= ctas) return;                    // the whole CTA: nothing waits for it
   const long long first = total * blockIdx.x / ctas;
   const int count = static_cast<int>(total * (blockIdx.x + 1) / ctas - first);
@@ -627,17 +626,17 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
 
 // Few requests, so up to all 148 parts of one: a CTA takes 64 channels, sixteen sets of sixteen threads
 // every sixteenth part, all of whose loads are issued before the factors that they wait for.
-__global__ void __launch_bounds__(256) decode_join_wide_kernel(const akl_decode_t c, const Work w, int hb_heads) {
+__device__ __forceinline__ void join_wide(const akl_decode_t& c, const Work& w, int hb_heads, int block) {
   constexpr int kSets = 16, kEach = kMaxCtas / kSets;
   __shared__ float sm_f[kMaxCtas];
   __shared__ float sm_red[16];
   __shared__ __align__(16) float sm_o[kSets][64];       // read and written as float4
-  const int b = blockIdx.x, head = blockIdx.y, ch0 = blockIdx.z * 64, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int head_of = block >> 2, b = head_of / c.q_heads, head = head_of - b * c.q_heads, ch0 = (block & 3) * 64;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long long row;
   const int n = request_of(c, b, row);
   const int hb = head / hb_heads, h = head - hb * hb_heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long at = static_cast<long long>(b) * c.q_heads + head;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + at * 256 + ch0;
   if (n == 0) {
@@ -703,16 +702,15 @@ __global__ void __launch_bounds__(256) decode_join_wide_kernel(const akl_decode_
 
 // Many requests, so few parts of each: a warp per (request, q head), a lane eight channels, one part
 // after the other with a running maximum.
-__global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, const Work w, int hb_heads) {
+__device__ __forceinline__ void join_warp(const akl_decode_t& c, const Work& w, int hb_heads, int block) {
   const int lane = threadIdx.x & 31;
-  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const long long at = static_cast<long long>(block) * 8 + (threadIdx.x >> 5);
   const bool in = at < static_cast<long long>(c.batch) * c.q_heads;
   const int b = in ? static_cast<int>(at / c.q_heads) : 0, head = in ? static_cast<int>(at - static_cast<long long>(b) * c.q_heads) : 0;
   const int hb = head / hb_heads, h = head - hb * hb_heads;
   long long row;
   const int n = request_of(c, b, row);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!in) return;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + at * 256 + lane * 8;
   float m = -INFINITY, l = 0.f, o[8];
@@ -752,25 +750,49 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const akl_decode_t c, 
   }
 }
 
-// weights[row][i] = decay weights[row][i] + sum_h 2^(x[h][i] - lse[h]), from the scores the decode
-// launch recorded: 4 bytes per position and q head written and read, against the K and V rows' 1024
-// per kv head.  A thread per position, 256 positions at a time.
-__global__ void __launch_bounds__(256) decode_weights_kernel(const akl_decode_t c, const Work w) {
+// weights[row][i] = decay weights[row][i] + sum_h 2^(x[h][i] - lse[h]), from the scores the decode launch
+// recorded: 4 bytes per position and q head written and read, against the K and V rows' 1024 per kv
+// head.  A thread per position, 256 positions at a time.  The log-sum-exps are put together here
+// once more from the parts (a few floats a head), so that this needs no launch behind the joins'.
+__device__ __forceinline__ void add_weights(const akl_decode_t& c, const Work& w, int hb_heads, int block, int blocks) {
   __shared__ long long sm_chunks[8];
   __shared__ float sm_lse[64];
-  const int b = blockIdx.x, tid = threadIdx.x;
+  const int b = block / blocks, part = block - b * blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long long row, before = 0;
   for (int i = tid; i < b; i += 256) before += (request_of(c, i, row) + kChunk - 1) / kChunk;
   before = warp_sum(before);
-  if ((tid & 31) == 0) sm_chunks[tid >> 5] = before;
+  if (lane == 0) sm_chunks[warp] = before;
   const int n = request_of(c, b, row);
+  if (part * 256 >= n) return;                        // the whole CTA
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid < c.q_heads) sm_lse[tid] = w.lse[static_cast<long long>(b) * c.q_heads + tid];
+  for (int head = warp; head < c.q_heads; head += 8) {
+    const int hb = head / hb_heads, h = head - hb * hb_heads;
+    const int4 info = w.info[b * 2 + hb];
+    const int parts = info.z - info.y + 1;
+    float lse;
+    if (parts == 1) {
+      lse = w.lse[static_cast<long long>(b) * c.q_heads + head];
+    } else {
+      float m = -INFINITY, l = 0.f;
+      for (int i = lane; i < parts; i += 32) {
+        const float2 ml = w.ml[(i == 0 ? info.x : 2 * (info.y + i)) * kSlotHeads + h];
+        const float top = fmaxf(m, ml.x), safe = top == -INFINITY ? 0.f : top;
+        l = l * ex2(m - safe) + ml.y * ex2(ml.x - safe);
+        m = top;
+      }
+      const float top = warp_max(m);
+      l *= ex2(m - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+      lse = l == 0.f ? -INFINITY : top + log2f(l);
+    }
+    if (lane == 0) sm_lse[head] = lse;
+  }
   __syncthreads();
   long long chunk0 = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) chunk0 += sm_chunks[i];
-  for (int i = blockIdx.y * 256 + tid; i < n; i += gridDim.y * 256) {
+  for (int i = part * 256 + tid; i < n; i += blocks * 256) {
     const long long chunk = chunk0 + i / kChunk;
     if (chunk >= w.max_chunks) {
       atomicCAS(w.status, 0, AKL_ERR_CAPACITY);
@@ -786,6 +808,15 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const akl_decode_t 
     float* dst = c.weights + row * c.weights_stride + i;
     *dst = c.weight_decay == 0.f ? total : fmaf(c.weight_decay, *dst, total);
   }
+}
+
+// What follows the decode launch: the joins, and behind them in the grid the weights.
+template <bool kWide>
+__global__ void __launch_bounds__(256) decode_finish_kernel(const akl_decode_t c, const Work w, int hb_heads, int joins, int blocks) {
+  const int block = blockIdx.x;
+  if (block >= joins) add_weights(c, w, hb_heads, block - joins, blocks);
+  else if (kWide) join_wide(c, w, hb_heads, block);
+  else join_warp(c, w, hb_heads, block);
 }
 
 int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
@@ -889,12 +920,14 @@ int akl_paged_decode(const akl_decode_t* c, void* stream) {
   if (rc != AKL_OK) return rc;
   // the wide join while its CTAs fit the GPU in about two waves; past that a request has few parts
   const int64_t pairs = static_cast<int64_t>(c->batch) * c->q_heads;
+  const bool wide = pairs * 4 <= 8 * sms;
+  const int64_t joins = wide ? pairs * 4 : (pairs + 7) / 8;
+  const int blocks = c->weights != nullptr ? std::min((c->table_width + 255) / 256, 64) : 0;
+  const int64_t grid = joins + static_cast<int64_t>(c->batch) * blocks;
+  if (grid >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
   const int hb_heads = hb * (c->q_heads / c->kv_heads);
-  rc = pairs * 4 <= 8 * sms ? launch_after(decode_join_wide_kernel, dim3(c->batch, c->q_heads, 4), s, "decode_join_wide_kernel", *c, w, hb_heads)
-                            : launch_after(decode_join_kernel, dim3(static_cast<unsigned>((pairs + 7) / 8)), s, "decode_join_kernel", *c, w, hb_heads);
-  if (rc != AKL_OK || c->weights == nullptr) return rc;
-  const int blocks = std::min((c->table_width + 255) / 256, 64);
-  return launch_after(decode_weights_kernel, dim3(c->batch, blocks), s, "decode_weights_kernel", *c, w);
+  return launch_after(wide ? decode_finish_kernel<true> : decode_finish_kernel<false>, dim3(static_cast<unsigned>(grid)), s,
+                      "decode_finish_kernel", *c, w, hb_heads, static_cast<int>(joins), blocks);
 }
 
 }  // extern "C"
