@@ -313,15 +313,19 @@ template <int HB>
 __device__ __forceinline__ void produce(const akl_decode_t& c, uint32_t smem, uint8_t* smem_gen, const Wait& wait,
                                         Cursor<HB>& at, long long first, int count, int own, int lane) {
   using T = Tile<HB>;
-  int slot[kAhead], block[kAhead];
-  // the page-table entry of this lane's position in the tile the cursor is at; -1: nothing to read
-  auto look = [&](int& s, int& hb) {
+  // The page-table entry of this lane's position in the tile the cursor is at, as it was loaded: anything that looks
+  // at it here, a sign extension even, would wait for the load (0.7 us a tile).  Negative: nothing to read.
+  int2 slot[kAhead];
+  int block[kAhead];
+  const bool wide = c.idx_dtype == AKL_IDX_I64;
+  auto look = [&](int2& s, int& hb) {
     hb = at.hb;
-    s = -1;
+    s = make_int2(-1, -1);
     const int i = at.t * T::kPos + own * T::kOwn + lane;
     if (lane < T::kOwn && i < at.n) {
-      const long long v = load_index(c.page_table, c.idx_dtype, at.row * c.table_stride + i);
-      if (v >= 0 && v < c.pool_rows) s = static_cast<int>(v);
+      const long long e = at.row * c.table_stride + i;
+      if (wide) s = __ldg(reinterpret_cast<const int2*>(c.page_table) + e);
+      else s.x = __ldg(reinterpret_cast<const int*>(c.page_table) + e);
     }
   };
   at.seek(first);
@@ -338,7 +342,8 @@ __device__ __forceinline__ void produce(const akl_decode_t& c, uint32_t smem, ui
     const int st = it % kStages;
     const bool free = it < kStages || (wait(bars + (kStages + st) * 8, ((it / kStages) - 1) & 1) && !*wait.aborted);
     if (!__all_sync(0xffffffffu, free)) break;
-    const int now = slot[0];
+    const bool there = slot[0].x >= 0 && slot[0].x < c.pool_rows && (!wide || slot[0].y == 0);
+    const int now = there ? slot[0].x : -1;
     const unsigned mask = __ballot_sync(0xffffffffu, now >= 0);
     const long long head0 = static_cast<long long>(block[0]) * (HB * 256) + lane * 8;
     const uint32_t dst = dst0 + st * T::kStage;
