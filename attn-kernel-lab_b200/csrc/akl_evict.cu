@@ -7,14 +7,17 @@
 // new place of a position then follows from two counts, of the positions before it that stay for
 // certain and of those with that key.
 //
-// A CTA, or a cluster of them while the requests leave SMs idle, takes a request; a thread holds up to 32 of its
-// weights in registers, so a row that fits is read once and written once, whatever the passes.  The
-// histograms and counts of a cluster meet through its shared memory.  Longer rows go through in rounds, their
-// weights read again for each digit (from L2).  Rows may be shortened in place: positions only move forward,
-// and what a group of 8192 positions a CTA overwrites has been read by all when its barrier opens.
+// A CTA, or a cluster of them while the requests leave SMs idle, takes a request and keeps the keys of up to
+// 32768 positions a CTA in shared memory, so a row that fits is read once and written once, whatever the
+// passes.  (In registers, 32 a thread, they were measured first: the unrolled loops spilled, 47 us instead
+// of 41.)  The histograms and counts of a cluster meet through its shared memory.  Longer rows go through in
+// rounds, their weights read again for each digit (from L2).  Rows may be shortened in place: positions only
+// move forward, and what a group of 8192 positions a CTA overwrites has been read by all when its barrier opens.
 //
-// Few bytes and two or three dependent passes: bound by the latency of the passes where requests are few, and
-// by the instructions per position where they are many, so the loops over a thread's positions have no branches.
+// Few bytes and two or three dependent passes.  One request of 139264 positions (16 CTAs) takes 20 us, of which
+// memory would be 0.5: two or three passes with two cluster barriers each, about a microsecond apiece, and the trips to
+// L2.  256 requests of up to 32768 take 41 us, memory 10: about 6 us a request whatever its length and 0.6 ns a
+// position, at 60 % of the issue slots.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -29,10 +32,11 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
-constexpr int kStep = 8, kGroups = 4;           // positions of a thread: groups of up to eight
+constexpr int kStep = 8, kGroups = 4;           // positions of a thread: groups of up to eight steps
 constexpr int kCap = kThreads * kStep * kGroups;
 constexpr int kMaxCluster = 16;
 constexpr int kBins = 2048;
+constexpr int kSorted = kThreads;              // requests that are put in order of their lengths, at most
 
 constexpr uint32_t kStays = 0xFFFFFFFFu;      // key of a position that stays whatever its weight; above every weight's
 constexpr uint32_t kNothing = 0u;              // key where there is no position; below every weight's
@@ -51,14 +55,39 @@ struct Shared {
   uint32_t counts[kGroups][kWarps];  // certain | equal << 16
   uint32_t totals[2][kGroups];     // of this CTA, by parity of the round; read by the cluster
   int warp_sums[kWarps];
+  int request;
 };
 
 template <typename Slot>
-__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c) {
+__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c, bool longest_first) {
   __shared__ __align__(16) Shared sm;
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int b = blockIdx.x / ctas;
+  if (longest_first) {                                  // as the b-th longest, of up to kSorted requests
+    int* lens = &sm.hist[0][0];
+    int* rank_of = &sm.hist[1][0];
+    for (int i = tid; i < c.batch; i += kThreads) {
+      lens[i] = static_cast<int>(max(0ll, min(static_cast<long long>(c.table_width), load_index(c.kv_lens, c.lens_dtype, i))));
+      rank_of[i] = 0;
+    }
+    __syncthreads();
+    int wide = kSorted;                                 // threads share a request's comparisons where there are enough
+    while (wide >= 2 * c.batch) wide >>= 1;
+    const int i = tid & (wide - 1), part = tid / wide, parts = kThreads / wide;
+    if (i < c.batch) {
+      const int mine = lens[i];
+      int longer = 0;
+#pragma unroll 4
+      for (int k = part; k < c.batch; k += parts) longer += lens[k] > mine || (lens[k] == mine && k < i) ? 1 : 0;
+      atomicAdd(&rank_of[i], longer);
+    }
+    __syncthreads();
+    if (tid < c.batch && rank_of[tid] == b) sm.request = tid;
+    __syncthreads();
+    b = sm.request;
+  }
   const unsigned before = (1u << lane) - 1u;
   const long long row = c.rows != nullptr ? load_index(c.rows, c.rows_dtype, b) : b;
   long long len = load_index(c.kv_lens, c.lens_dtype, b);
@@ -79,62 +108,62 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
   auto key_of = [&](float w, int i) { return i >= n ? kNothing : (i < low || i >= high ? kStays : weight_key(w)); };
 
   // A group is side by side in the row, in it a CTA's share, in it a warp's: `each` steps of 32 positions.
-  uint32_t key[kGroups][kStep];
+  extern __shared__ uint32_t keys[];                    // [groups][warps][each][32]
   int each = 0, groups = 0, base = 0;
-  unsigned alike = 0, odd = 0;                          // groups of which the warp's keys are all one; some are not the weight's bits
+  // groups of which the warp has positions; whose keys are all one; some of whose keys are not the weight's bits
+  unsigned present = 0, alike = 0, odd = 0;
   auto start_of = [&](int g) { return base + ((g * ctas + rank) * kWarps + warp) * each * 32 + lane; };
+  auto keys_of = [&](int g) { return keys + (g * kWarps + warp) * (kStep * 32) + lane; };
   auto load = [&]() {
     const int left = min(per_round, n - base), wide = (left + ctas * kThreads - 1) / (ctas * kThreads);
     each = min(kStep, wide);
     groups = (wide + each - 1) / each;
-    alike = odd = 0;
+    present = alike = odd = 0;
+#pragma unroll 2
+    for (int g = 0; g < groups; ++g) {
+      const int at = start_of(g), from = at - lane, to = from + each * 32;
+      if (from >= n) break;
+      present |= 1u << g;
+      const float* src = weights + at;
+      uint32_t key[kStep];
+      if (each == kStep && to <= n) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g)                   // the weights' bits first, so that all the loads are in flight
-      if (g < groups) {
-        const int at = start_of(g);
-        const float* from = weights + at;
-        if (each == kStep && at - lane + kStep * 32 <= n) {
+        for (int k = 0; k < kStep; ++k) key[k] = __float_as_uint(src[k * 32]);
+      } else {
 #pragma unroll
-          for (int k = 0; k < kStep; ++k) key[g][k] = __float_as_uint(from[k * 32]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) key[g][k] = k < each && at + k * 32 < n ? __float_as_uint(from[k * 32]) : 0u;
-        }
-        // the slots are wanted behind the passes: have them in L2 by then
-        const int line = at - lane + lane * static_cast<int>(128 / sizeof(Slot));
-        if (lane * static_cast<int>(128 / sizeof(Slot)) < each * 32 && line < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(slots + line));
+        for (int k = 0; k < kStep; ++k) key[k] = k < each && at + k * 32 < n ? __float_as_uint(src[k * 32]) : 0u;
       }
+      // the slots are wanted behind the passes: have them in L2 by then
+      const int line = from + lane * static_cast<int>(128 / sizeof(Slot));
+      if (line < min(to, n)) asm volatile("prefetch.global.L2 [%0];" ::"l"(slots + line));
+      uint32_t most = key[0], least = key[0];
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (g < groups) {
-        const int at = start_of(g), from = at - lane, to = from + each * 32;
-        uint32_t least = key[g][0], most = key[g][0];
-#pragma unroll
-        for (int k = 1; k < kStep; ++k) {
-          least = min(least, key[g][k]);
-          most = max(most, key[g][k]);
-        }
-        // weights that are at least 0 and no NaN, in positions that compete, are their own order
-        if (__all_sync(0xffffffffu, most <= 0x7F800000u) && from >= low && to <= high && each == kStep) {
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) key[g][k] |= 0x80000000u;
-          const uint32_t first = __shfl_sync(0xffffffffu, least, 0);
-          if (__all_sync(0xffffffffu, least == first && most == first)) alike |= 1u << g;
-        } else {
-          bool strange = false, same = true;
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) {
-            const uint32_t bits = key[g][k];
-            key[g][k] = k < each ? key_of(__uint_as_float(bits), at + k * 32) : kNothing;
-            strange |= key[g][k] != kNothing && __float_as_uint(key_weight(key[g][k])) != bits;
-          }
-          const uint32_t first = __shfl_sync(0xffffffffu, key[g][0], 0);
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) same &= key[g][k] == first || k >= each;
-          if (__all_sync(0xffffffffu, same)) alike |= 1u << g;
-          if (__any_sync(0xffffffffu, strange)) odd |= 1u << g;
-        }
+      for (int k = 1; k < kStep; ++k) {
+        most = max(most, key[k]);
+        least = min(least, key[k]);
       }
+      uint32_t* dst = keys_of(g);
+      // weights that are at least 0 and no NaN, in positions that compete, are their own order
+      if (each == kStep && from >= low && to <= high && __all_sync(0xffffffffu, most <= 0x7F800000u)) {
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) dst[k * 32] = key[k] | 0x80000000u;
+      } else {
+        bool strange = false;
+        least = 0xFFFFFFFFu;
+        most = 0u;
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+          const uint32_t bits = key[k];
+          key[k] = k < each ? key_of(__uint_as_float(bits), at + k * 32) : kNothing;
+          strange |= key[k] != kNothing && __float_as_uint(key_weight(key[k])) != bits;
+          dst[k * 32] = key[k];
+          if (k < each) { most = max(most, key[k]); least = min(least, key[k]); }
+        }
+        if (__any_sync(0xffffffffu, strange)) odd |= 1u << g;
+      }
+      const uint32_t first = __shfl_sync(0xffffffffu, least, 0);
+      if (__all_sync(0xffffffffu, least == first && most == first)) alike |= 1u << g;
+    }
   };
   if (!idle && n > 0 && once) load();
 
@@ -145,7 +174,9 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
     if (ctas > 1) cluster.barrier_arrive();             // waited for before anybody adds to the first CTA's counts
     uint32_t prefix = 0;
     bool exact = false;                                 // every key that begins with prefix stays
-    for (int pass = 0; pass < 3 && !exact; ++pass) {
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      if (exact) break;
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
       int* hist = sm.hist[pass];
       const uint32_t mask = (1u << bits) - 1u;
@@ -154,18 +185,17 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
         if (pass == 0 ? k != kNothing : (d >> bits) == prefix) atomicAdd(&hist[d & mask], 1);
       };
       if (once) {
+        for (int g = 0; g < groups && ((present >> g) & 1u) != 0u; ++g) {
+          const uint32_t* key = keys_of(g);
+          if ((alike >> g) & 1u) {
+            // one key (of weights that nobody has added to yet): one lane adds for all, or 32 would queue
+            const uint32_t d = key[0] >> shift;
+            if (lane == 0 && (pass == 0 ? key[0] != kNothing : (d >> bits) == prefix)) atomicAdd(&hist[d & mask], 32 * each);
+          } else {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-          if (g < groups) {
-            if ((alike >> g) & 1u) {
-              // one key (of weights that nobody has added to yet): one lane adds for all, or 32 would queue
-              const uint32_t d = key[g][0] >> shift;
-              if (lane == 0 && (pass == 0 ? key[g][0] != kNothing : (d >> bits) == prefix)) atomicAdd(&hist[d & mask], 32 * each);
-            } else {
-#pragma unroll
-              for (int k = 0; k < kStep; ++k) add(key[g][k]);
-            }
+            for (int k = 0; k < kStep; ++k) add(key[k * 32]);
           }
+        }
       } else {
         const int step = ctas * kThreads;
         for (int at = rank * kThreads + tid; at < n; at += kStep * step) {
@@ -224,16 +254,19 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
   int certain0 = 0, equal0 = 0;                         // in the groups before
   for (int round = 0; base < n && !idle; base += per_round, ++round) {
     if (!once) load();
-    uint32_t mine[kGroups];                             // of this warp: certain | equal << 16
+    for (int g = 0; g < groups; ++g) {
+      uint32_t count = 0;
+      if ((present >> g) & 1u) {
+        const uint32_t* key = keys_of(g);
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (g < groups) {
-        uint32_t count = 0;
-#pragma unroll
-        for (int k = 0; k < kStep; ++k) count += (key[g][k] > threshold ? 1u : 0u) + (key[g][k] == threshold ? 0x10000u : 0u);
-        mine[g] = __reduce_add_sync(0xffffffffu, count);
-        if (lane == 0) sm.counts[g][warp] = mine[g];
+        for (int k = 0; k < kStep; ++k) {
+          const uint32_t v = key[k * 32];
+          count += (v > threshold ? 1u : 0u) + (v == threshold ? 0x10000u : 0u);
+        }
+        count = __reduce_add_sync(0xffffffffu, count);
       }
+      if (lane == 0) sm.counts[g][warp] = count;
+    }
     __syncthreads();
     if (ctas > 1) {
       if (warp < groups) {
@@ -242,19 +275,24 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
       }
       cluster.sync();                                   // every weight of the round is in a register
     }
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-      if (g < groups) {
+    for (int g = 0; g < groups; ++g) {
         const int at = start_of(g);
+        const bool some = ((present >> g) & 1u) != 0u, again = ((odd >> g) & 1u) != 0u;
         Slot slot[kStep];
         float w[kStep];
-        const bool again = ((odd >> g) & 1u) != 0u;
+        uint32_t key[kStep];
+        if (some) {
+          const Slot* from = slots + at;
+          const uint32_t* src = keys_of(g);
 #pragma unroll
-        for (int k = 0; k < kStep; ++k) {
-          w[k] = key_weight(key[g][k]);
-          if (key[g][k] != kNothing) {
-            slot[k] = slots[at + k * 32];
-            if (again) w[k] = weights[at + k * 32];
+          for (int k = 0; k < kStep; ++k) {
+            key[k] = src[k * 32];
+            if (key[k] != kNothing) slot[k] = from[k * 32];
+          }
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            w[k] = key_weight(key[k]);
+            if (again && key[k] != kNothing) w[k] = weights[at + k * 32];
           }
         }
         const uint32_t count = sm.counts[g][lane];
@@ -275,22 +313,23 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
           equal0 += static_cast<int>(total >> 16);
           if (in_place) __syncthreads();
         }
-        if ((mine[g] >> 16) == 0u) {                    // no key of the warp equals the threshold
+        if (!some) continue;
+        if ((sm.counts[g][warp] >> 16) == 0u) {         // no key of the warp equals the threshold
           const int equals = min(equal, need);
 #pragma unroll
           for (int k = 0; k < kStep; ++k) {
-            const bool stay = key[g][k] > threshold;
+            const bool stay = key[k] > threshold;
             const unsigned stays = __ballot_sync(0xffffffffu, stay);
             const int to = certain + equals + __popc(stays & before);
             certain += __popc(stays);
             if (stay) slots_out[to] = slot[k];
             if (stay) weights_out[to] = w[k];
-            if (!stay && key[g][k] != kNothing) freed[at + k * 32 - to] = slot[k];
+            if (!stay && key[k] != kNothing) freed[at + k * 32 - to] = slot[k];
           }
         } else {
 #pragma unroll
           for (int k = 0; k < kStep; ++k) {
-            const bool sure = key[g][k] > threshold, same = key[g][k] == threshold;
+            const bool sure = key[k] > threshold, same = key[k] == threshold;
             const unsigned sures = __ballot_sync(0xffffffffu, sure), sames = __ballot_sync(0xffffffffu, same);
             const int rank_same = equal + __popc(sames & before);
             const int to = certain + __popc(sures & before) + min(rank_same, need);
@@ -299,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
             equal += __popc(sames);
             if (stay) slots_out[to] = slot[k];
             if (stay) weights_out[to] = w[k];
-            if (!stay && key[g][k] != kNothing) freed[at + k * 32 - to] = slot[k];
+            if (!stay && key[k] != kNothing) freed[at + k * 32 - to] = slot[k];
           }
         }
       }
@@ -317,12 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c)
 }
 
 template <typename Slot>
-int launch_evict(const akl_evict_t& c, int ctas, cudaStream_t s) {
+int launch_evict(const akl_evict_t& c, int ctas, bool longest_first, cudaStream_t s) {
   static std::atomic<bool> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire))) {
     e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCap * 4);
     if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute attr;
@@ -332,10 +372,11 @@ int launch_evict(const akl_evict_t& c, int ctas, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * ctas);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kCap * 4;
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, evict_kernel<Slot>, c);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, evict_kernel<Slot>, c, longest_first);
   if (e != cudaSuccess) { note_cuda_error(e, "evict_kernel"); return AKL_ERR_CUDA; }
   return AKL_OK;
 }
@@ -370,5 +411,11 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
   int ctas = 1;
   while (ctas < kMaxCluster && static_cast<int64_t>(c->batch) * ctas * 2 <= sms && c->table_width > 2 * kThreads * ctas) ctas *= 2;
   if (static_cast<int64_t>(c->batch) * ctas >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
-  return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, ctas, s) : launch_evict<int>(*c, ctas, s);
+  // More requests than SMs: the long ones first, or the last to start could be the longest (47 us became 41).
+  // Every CTA then reads all lengths, so not where the first ones to finish overwrite them.
+  const int64_t lens_bytes = static_cast<int64_t>(c->batch) * (c->lens_dtype == AKL_IDX_I64 ? 8 : 4);
+  const int64_t apart = static_cast<const char*>(c->kv_lens_out) - static_cast<const char*>(c->kv_lens);
+  const bool longest_first = ctas == 1 && c->batch > sms && c->batch <= kSorted && (apart >= lens_bytes || -apart >= lens_bytes);
+  return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, ctas, longest_first, s)
+                                     : launch_evict<int>(*c, ctas, longest_first, s);
 }

@@ -397,6 +397,10 @@ def test_eviction_rows_strides_and_lengths_out_of_range(pkg, cuda, in_place):
               keep=20, protect_first=2, protect_last=5)
     many, wm = evict_case([300] * 200, 300, seed=4)
     run_evict(pkg, many, wm, [(7 * i) % 301 for i in range(200)], in_place=in_place, keep=100, protect_last=10)
+    # more requests than SMs, nearly all of them shortened: nobody may go by a length that another one wrote
+    crowd, wc = evict_case([300] * 400, 300, seed=5)
+    run_evict(pkg, crowd, wc, [90 + (37 * i) % 211 for i in range(400)], in_place=in_place, keep=100, protect_first=3)
+    run_evict(pkg, torch.cat([crowd] * 3), torch.cat([wc] * 3), [300 - (i % 7) for i in range(1200)], in_place=in_place, keep=64)
     # rows of larger tables
     big = torch.zeros((9, 200), dtype=I64, device=cuda)
     acc = torch.full((9, 130), 7.0, device=cuda)
