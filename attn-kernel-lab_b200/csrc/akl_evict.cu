@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
   } else {
     need = 0x7fffffff;
   }
-  const bool in_place = static_cast<const void*>(slots_out) == static_cast<const void*>(slots);
+  // (some weights are read again next to their slots, so either one in place needs the barrier)
+  const bool in_place = slots_out == slots || weights_out == weights;
 
   int certain0 = 0, equal0 = 0;                         // in the groups before
   for (int round = 0; base < n && !idle; base += per_round, ++round) {
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
           equal += __reduce_add_sync(0xffffffffu, lane < rank ? theirs_e : 0);
           certain0 += __reduce_add_sync(0xffffffffu, theirs_c);
           equal0 += __reduce_add_sync(0xffffffffu, theirs_e);
-          if (in_place) cluster.sync();                 // every slot of the group has been read
+          if (in_place) cluster.sync();                 // every slot and weight of the group has been read
         } else {
           const uint32_t total = __reduce_add_sync(0xffffffffu, count);
           certain0 += static_cast<int>(total & 0xFFFFu);

@@ -414,6 +414,21 @@ def test_eviction_rows_strides_and_lengths_out_of_range(pkg, cuda, in_place):
     assert not big[:, :60].any() and not big[:, 140:].any() and bool((acc[:, :21] == 7).all() and (acc[:, 101:] == 7).all())
 
 
+@pytest.mark.parametrize("part", ["table", "weights"])
+def test_eviction_with_one_output_in_place(pkg, cuda, part):
+    """The table alone, or the weights alone, in place; weights that are read a second time (NaN, -0) among them."""
+    for lens, width, keep in (([30000, 777, 9000], 30003, 4000), ([70001], 70001, 30000)):
+        table, w = evict_case(lens, width, kind="odd", seed=width)
+        want = R.evict(table, w, lens, keep, 5, 70)
+        for _ in range(3):
+            t, a, n = table.to(cuda), w.to(cuda), torch.tensor(lens, dtype=I32, device=cuda)
+            outs = dict(weights_out=a.clone()) if part == "table" else dict(page_table_out=t.clone())
+            got = pkg.evict_lightest(t, a, n, keep=keep, protect_first=5, protect_last=70, **outs)
+            assert torch.equal(got[0].cpu(), want[0]) and n.tolist() == want[2]
+            assert torch.equal(got[1].cpu().view(torch.int32), want[1].view(torch.int32))
+            assert (got[0] is t) == (part == "table") and (got[1] is a) == (part == "weights")
+
+
 def test_eviction_in_a_graph_reads_lengths_at_replay(pkg, cuda):
     table, w = evict_case([500, 400], 512, seed=6)
     t, a, n = table.to(cuda), w.to(cuda), torch.tensor([500, 400], dtype=I32, device=cuda)
