@@ -15,8 +15,8 @@
 //     instruction, with the page-table entries four tiles ahead.  Rows lie 16 bytes off a multiple of 128 in
 //     shared memory, so that matrix loads meet no bank twice.  (Bulk copies of a row each were measured
 //     first: about 75 cycles of the copy unit apiece, 94 us for 136 MB in rows of 512 bytes.)
-//   * eight warps: four (kv head, 16 positions) tasks times two halves of the output channels.  Both
-//     halves form the scores, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
+//   * eight warps: four (kv head, 16 positions) tasks times two halves of the channels.  A pair of warps
+//     forms the scores, half the products each, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
 //     heads of the kv head on N -- with the heads on M half to three quarters of the tensor work would
 //     be padding.  Out^T = V^T P^T takes P^T in the operand layout that an 8x8 transpose of the score
 //     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: a tile needs 8192
@@ -72,8 +72,9 @@ struct Tile {
   static constexpr int kMerge = kGroups > 1 ? 16384 : 0;
   static constexpr int kOffMerge = kRing;
   static constexpr int kOffMl = kOffMerge + kMerge;  // [8 warps][8 heads] {m, l}
+  static constexpr int kOffMeet = kOffMl + 512;      // [2][8 warps][32 lanes] float4: half scores of a warp for its partner
   static constexpr int kOwn = kPos / kProducers;     // positions of a tile that one producer warp gathers
-  static constexpr int kOffMask = kOffMl + 512;      // [kStages][kProducers] u32: which of them are there
+  static constexpr int kOffMask = kOffMeet + 8192;      // [kStages][kProducers] u32: which of them are there
   static constexpr int kOffBar = kOffMask + 16 * kStages;
   static constexpr int kSmem = kOffBar + 16 * kStages + 16;
 };
@@ -268,25 +269,27 @@ __device__ __forceinline__ uint32_t split2(float a, float b, uint32_t& rest) {
   return hi;
 }
 
-// Queries of one kv head as the B operand: thread (g, q) = (lane / 4, lane % 4) holds head g, channels
-// 16 k + 2 q, + 1 and the same + 8.  cs: what scores of the heads 2 q and 2 q + 1 are multiplied by.
+// Queries of one kv head as the B operand, channels 128 half ..: thread (g, q) = (lane / 4, lane % 4) holds head g,
+// channels 16 k + 2 q, + 1 and the same + 8.  cs: what scores of the heads 2 q and 2 q + 1 are multiplied by.
 template <int KV>
-__device__ __forceinline__ void load_q(const akl_decode_t& c, int b, int head0, int group, int lane, uint32_t (&q)[16][2], float (&cs)[2]) {
+__device__ __forceinline__ void load_q(const akl_decode_t& c, int b, int head0, int group, int half, int lane, uint32_t (&q)[8][2], float (&cs)[2]) {
   const int g = lane >> 2, quad = lane & 3;
   const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(c.q) + b * c.q_stride + (head0 + g) * 256) + quad;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    q[k][0] = g < group ? __ldg(src + k * 8) : 0u;
-    q[k][1] = g < group ? __ldg(src + k * 8 + 4) : 0u;
+  for (int k = 0; k < 8; ++k) {
+    q[k][0] = g < group ? __ldg(src + half * 64 + k * 8) : 0u;
+    q[k][1] = g < group ? __ldg(src + half * 64 + k * 8 + 4) : 0u;
   }
   cs[0] = cs[1] = c.sm_scale * kLog2e;
   if (KV == AKL_KV_FP16) {
     float top = 0.f;
+    auto larger = [&](uint32_t v) { top = fmaxf(top, fmaxf(fabsf(bf16_bits_to_float(v & 0xFFFFu)), fabsf(bf16_bits_to_float(v >> 16)))); };
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        top = fmaxf(top, fmaxf(fabsf(bf16_bits_to_float(q[k][e] & 0xFFFFu)), fabsf(bf16_bits_to_float(q[k][e] >> 16))));
+    for (int k = 0; k < 8; ++k) {
+      larger(q[k][0]);
+      larger(q[k][1]);
+      larger(g < group ? __ldg(src + (half ^ 1) * 64 + k * 8) : 0u);
+      larger(g < group ? __ldg(src + (half ^ 1) * 64 + k * 8 + 4) : 0u);
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -296,7 +299,7 @@ __device__ __forceinline__ void load_q(const akl_decode_t& c, int b, int head0, 
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < 8; ++k) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const __half2 h = __floats2half2_rn(bf16_bits_to_float(q[k][i] & 0xFFFFu) * down, bf16_bits_to_float(q[k][i] >> 16) * down);
@@ -420,17 +423,18 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   const int g = lane >> 2, quad = lane & 3, group = c.q_heads / c.kv_heads;
   const uint32_t bars = smem + T::kOffBar;
   constexpr float kShift = KV == AKL_KV_FP16 ? 14.f : 0.f;   // P carries 2^kShift
-  const uint32_t k_lane = (tg * 16 + (lane & 15)) * T::kPitch + unit * 512 + (lane >> 4) * 16;
+  const uint32_t k_lane = (tg * 16 + (lane & 15)) * T::kPitch + unit * 512 + half * 256 + (lane >> 4) * 16;
   const uint32_t v_lane = T::kPlane + (tg * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * T::kPitch + unit * 512 + half * 256 +
                           ((lane >> 3) & 1) * 16;
-  uint32_t q[16][2];
+  float4* const meet = reinterpret_cast<float4*>(smem_gen + T::kOffMeet) + lane;      // [tile & 1][warp][lane]
+  uint32_t q[8][2];
   float cs[2], m[2], l[2], o[8][4];
   bool ok = true, new_piece = true;
   int t_begin = 0;
   at.seek(first);
   for (int it = 0; it < count; ++it) {
     if (new_piece) {
-      load_q<KV>(c, at.b, (at.hb * HB + unit) * group, group, lane, q, cs);
+      load_q<KV>(c, at.b, (at.hb * HB + unit) * group, group, half, lane, q, cs);
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
 #pragma unroll
@@ -441,26 +445,39 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
     const int st = it % kStages;
     const uint32_t stage = smem + st * T::kStage;
     if (ok) ok = __all_sync(0xffffffffu, wait(bars + st * 8, (it / kStages) & 1));
+    unsigned there = 0;                 // positions of this warp's sixteen that are there
     if (ok) {
-      unsigned there = 0;               // positions of this warp's sixteen that are there
 #pragma unroll
       for (int i = 0; i < 16 / T::kOwn; ++i)
         there |= reinterpret_cast<volatile uint32_t*>(smem_gen + T::kOffMask + st * 16)[tg * (16 / T::kOwn) + i] << (i * T::kOwn);
-      // scores of 16 positions x 8 heads: thread has positions g, g + 8 of heads 2 quad, 2 quad + 1.
-      // Four chains of four products keep the sums short, in time and in rounding.
-      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    }
+    // Scores of 16 positions x 8 heads: thread has positions g, g + 8 of heads 2 quad, 2 quad + 1.  Each of the
+    // pair of warps multiplies half the channels; two chains keep the sums short, in time and in rounding.
+    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float4* const buf = meet + (it & 1) * (kWarps * 32);    // its next use is two tiles on, behind the next tile's barrier
+    float4 own = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there != 0u) {
+      float s[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t a[4];
+        ldsm4(stage + k_lane + k * 32, a);
+        mma16<KV>(s[k & 1], a, q[k][0], q[k][1]);
+      }
+      own = make_float4(s[0][0] + s[1][0], s[0][1] + s[1][1], s[0][2] + s[1][2], s[0][3] + s[1][3]);
+      buf[warp * 32] = own;
+    }
+    // (by every warp for every tile, whatever it found: nobody waits here for one that gave up)
+    asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
+    if (ok) {
       if (there != 0u) {
-        float s[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          uint32_t a[4];
-          ldsm4(stage + k_lane + k * 32, a);
-          mma16<KV>(s[k & 3], a, q[k][0], q[k][1]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = ((s[0][i] + s[1][i]) + (s[2][i] + s[3][i])) * cs[i & 1];
+        const float4 other = buf[(warp ^ 4) * 32];
+        x[0] = (own.x + other.x) * cs[0];
+        x[1] = (own.y + other.y) * cs[1];
+        x[2] = (own.z + other.z) * cs[0];
+        x[3] = (own.w + other.w) * cs[1];
         if (there != 0xFFFFu) {
           if (!((there >> g) & 1u)) x[0] = x[1] = -INFINITY;
           if (!((there >> (g + 8)) & 1u)) x[2] = x[3] = -INFINITY;
@@ -535,6 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
 
     // ---- end of this CTA's piece of (request, head block)
     new_piece = true;
+    if (*wait.aborted) ok = false;
+    ok = __all_sync(0xffffffffu, ok);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
