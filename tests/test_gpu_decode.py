@@ -223,6 +223,22 @@ def test_decode_on_two_streams_with_two_workspaces(pkg, cuda):
         assert all(torch.equal(alone, o) for o in outs[i])
 
 
+def test_decode_of_thousands_of_short_requests(pkg, cuda):
+    lens = [(31 * i) % 43 for i in range(2500)]
+    run_decode(pkg, R.case(lens, 1, 1, seed=40), decay=1.0)
+    # more requests than a warp's window of lengths, nearly all of them empty
+    lens = [0] * 700 + [300] + [0] * 500 + [5, 0, 17]
+    run_decode(pkg, R.case(lens, 2, 2, dtype=FP16, seed=41), decay=0.0)
+
+
+def test_decode_rows_may_repeat_without_weights(pkg, cuda):
+    c = R.case([500, 80], 24, 4, seed=42)
+    c["rows"] = c["rows"][:1].repeat(3)
+    c["kv_lens"] = torch.tensor([500, 500, 123], dtype=I32, device=cuda)
+    c["q"] = torch.cat([c["q"][:1], c["q"]])
+    run_decode(pkg, c)
+
+
 # ---- attention weights of an extend ---------------------------------------------------------------
 def extend_case(rows, prefix, q_heads, kv_heads, *, dtype=BF16, idx=I32, extra=0, seed=0, gain=1.0):
     """`extra` positions lie behind the last row's diagonal: nobody sees them, and their keys are NaN."""
@@ -446,6 +462,54 @@ def test_eviction_in_a_graph_reads_lengths_at_replay(pkg, cuda):
         want = R.evict(table, w, lens, 128, 3, 0)
         assert torch.equal(outs["page_table_out"].cpu(), want[0]) and torch.equal(outs["weights_out"].cpu(), want[1])
         assert outs["kv_lens_out"].tolist() == want[2] and counts.tolist() == [len(f) for f in want[3]]
+
+
+def test_extend_weights_and_eviction_on_two_streams(pkg, cuda):
+    """Their own workspaces, or none: nothing is shared between streams, and clusters of both fit side by side."""
+    extends = [extend_case(90, 700, 24, 4, seed=50), extend_case(40, 1500, 24, 4, dtype=FP16, seed=51)]
+    spaces = [pkg.plan_weights_workspace(cuda, max_kv_len=1600, max_q_len=90, q_heads=24, kv_heads=4) for _ in extends]
+    evicts = [evict_case([40000], 40000, seed=52), evict_case([9000, 8000], 9000, seed=53)]
+    tables = [[t.to(cuda) for t in e] for e in evicts]
+    lens = [torch.tensor(n, dtype=I32, device=cuda) for n in ([40000], [9000, 8000])]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                w = torch.zeros(extends[i]["idx"].shape[0], device=cuda)
+                pkg.extend_weights(**extends[i], weights=w, workspace=spaces[i])
+                t, a, n = tables[i][0].clone(), tables[i][1].clone(), lens[i].clone()
+                pkg.evict_lightest(t, a, n, keep=700, protect_last=9)
+                got[i].append((w, t, a, n))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        ref, tol = R.extend_weights(*(extends[i][k] for k in ("q", "k_pool", "idx", "prefix", "lse")), torch.zeros_like(got[i][0][0]))
+        want = R.evict(*evicts[i], lens[i].tolist(), 700, 0, 9)
+        for w, t, a, n in got[i]:
+            R.within(w, ref, tol)
+            assert torch.equal(w, got[i][0][0])
+            assert torch.equal(t.cpu(), want[0]) and torch.equal(a.cpu(), want[1]) and n.tolist() == want[2]
+
+
+def test_eviction_of_long_rows_in_a_graph(pkg, cuda):
+    """Clusters of CTAs, in place, replayed: the second replay finds short rows and leaves them."""
+    table, w = evict_case([60000, 20000], 60000, seed=60)
+    t, a, n = table.to(cuda), w.to(cuda), torch.tensor([60000, 20000], dtype=I64, device=cuda)
+    freed, counts = torch.zeros((2, 60000), dtype=I32, device=cuda), torch.zeros(2, dtype=I32, device=cuda)
+    scratch = (t.clone(), a.clone(), n.clone())
+    pkg.evict_lightest(*scratch, keep=5000, protect_first=1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.evict_lightest(t, a, n, keep=5000, protect_first=1, freed=freed, freed_lens=counts)
+    want = R.evict(table, w, [60000, 20000], 5000, 1, 0)
+    graph.replay()
+    assert counts.tolist() == [55000, 15000] and freed[0, :55000].tolist() == want[3][0]
+    for _ in range(2):
+        assert torch.equal(t.cpu(), want[0]) and torch.equal(a.cpu(), want[1]) and n.tolist() == [5000, 5000]
+        graph.replay()
+        assert counts.tolist() == [0, 0]
 
 
 # ---- together --------------------------------------------------------------------------------------
