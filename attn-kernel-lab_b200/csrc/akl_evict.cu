@@ -66,10 +66,12 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int b = blockIdx.x / ctas;
   if (longest_first) {                                  // as the b-th longest, of up to kSorted requests
-    int* lens = &sm.hist[0][0];
+    // lengths and, where they are equal, the lower index first, as one number; rank by counting the larger ones
+    int* order = &sm.hist[0][0];
     int* rank_of = &sm.hist[1][0];
-    for (int i = tid; i < c.batch; i += kThreads) {
-      lens[i] = static_cast<int>(max(0ll, min(static_cast<long long>(c.table_width), load_index(c.kv_lens, c.lens_dtype, i))));
+    const int padded = (c.batch + 15) & ~15;
+    for (int i = tid; i < padded; i += kThreads) {
+      order[i] = i < c.batch ? static_cast<int>(max(0ll, min(static_cast<long long>(c.table_width), load_index(c.kv_lens, c.lens_dtype, i)))) * kSorted + (kSorted - 1 - i) : -1;
       rank_of[i] = 0;
     }
     __syncthreads();
@@ -77,11 +79,15 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
     while (wide >= 2 * c.batch) wide >>= 1;
     const int i = tid & (wide - 1), part = tid / wide, parts = kThreads / wide;
     if (i < c.batch) {
-      const int mine = lens[i];
-      int longer = 0;
+      const int mine = order[i];
+      int larger = 0;
 #pragma unroll 4
-      for (int k = part; k < c.batch; k += parts) longer += lens[k] > mine || (lens[k] == mine && k < i) ? 1 : 0;
-      atomicAdd(&rank_of[i], longer);
+      for (int k = part * 4; k < padded; k += parts * 4) {
+        const int4 v = *reinterpret_cast<const int4*>(order + k);
+        larger += (v.x > mine ? 1 : 0) + (v.y > mine ? 1 : 0) + (v.z > mine ? 1 : 0) + (v.w > mine ? 1 : 0);
+      }
+      if (parts > 1) atomicAdd(&rank_of[i], larger);
+      else rank_of[i] = larger;
     }
     __syncthreads();
     if (tid < c.batch && rank_of[tid] == b) sm.request = tid;
@@ -416,7 +422,7 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
   // Every CTA then reads all lengths, so not where the first ones to finish overwrite them.
   const int64_t lens_bytes = static_cast<int64_t>(c->batch) * (c->lens_dtype == AKL_IDX_I64 ? 8 : 4);
   const int64_t apart = static_cast<const char*>(c->kv_lens_out) - static_cast<const char*>(c->kv_lens);
-  const bool longest_first = ctas == 1 && c->batch > sms && c->batch <= kSorted && (apart >= lens_bytes || -apart >= lens_bytes);
+  const bool longest_first = ctas == 1 && c->batch > sms && c->batch <= kSorted && c->table_width < (1 << 21) && (apart >= lens_bytes || -apart >= lens_bytes);
   return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, ctas, longest_first, s)
                                      : launch_evict<int>(*c, ctas, longest_first, s);
 }
