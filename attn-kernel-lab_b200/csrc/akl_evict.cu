@@ -10,13 +10,13 @@
 // A CTA, or a cluster of them while the requests leave SMs idle, takes a request and keeps the keys of up to
 // 32768 positions a CTA in shared memory, so a row that fits is read once and written once, whatever the
 // passes.  (In registers, 32 a thread, they were measured first: the unrolled loops spilled, 47 us instead
-// of 41.)  The histograms and counts of a cluster meet through its shared memory.  Longer rows go through in
+// of 41 then.)  The histograms and counts of a cluster meet through its shared memory.  Longer rows go through in
 // rounds, their weights read again for each digit (from L2).  Rows may be shortened in place: positions only
 // move forward, and what a group of 8192 positions a CTA overwrites has been read by all when its barrier opens.
 //
 // Few bytes and two or three dependent passes.  One request of 139264 positions (16 CTAs) takes 20 us, of which
 // memory would be 0.5: two or three passes with two cluster barriers each, about a microsecond apiece, and the trips to
-// L2.  256 requests of up to 32768 take 41 us, memory 10: about 6 us a request whatever its length and 0.6 ns a
+// L2.  256 requests of up to 32768 take 38 us, memory 10: about 6 us a request whatever its length and 0.6 ns a
 // position, at 60 % of the issue slots.
 #include <cooperative_groups.h>
 
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
       else __syncthreads();
       const int4 found = *cluster.map_shared_rank(&sm.found[pass], 0);
       prefix = (prefix << bits) | static_cast<uint32_t>(found.x);
-      need = found.y;
+      need = max(0, found.y);
       exact = found.z != 0;
       threshold = prefix << shift;
     }
@@ -321,6 +321,13 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
           if (in_place) __syncthreads();
         }
         if (!some) continue;
+        // Weights that were read again for each digit agree with what is moved only while nobody else writes them, which
+        // a row that two requests name breaks: what is listed as freed must still end inside the request's own entries.
+        if (!once && full) {
+          const uint32_t mine = sm.counts[g][warp];
+          const int upto = min(n, at - lane + each * 32);
+          if (upto - certain - static_cast<int>(mine & 0xFFFFu) - min(equal + static_cast<int>(mine >> 16), need) > n - c.keep) continue;
+        }
         if ((sm.counts[g][warp] >> 16) == 0u) {         // no key of the warp equals the threshold
           const int equals = min(equal, need);
 #pragma unroll
@@ -418,7 +425,8 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
   int ctas = 1;
   while (ctas < kMaxCluster && static_cast<int64_t>(c->batch) * ctas * 2 <= sms && c->table_width > 2 * kThreads * ctas) ctas *= 2;
   if (static_cast<int64_t>(c->batch) * ctas >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
-  // More requests than SMs: the long ones first, or the last to start could be the longest (47 us became 41).
+  // More requests than SMs: the long ones first, or the last to start could be the longest (47 us became 41, and 38 with
+  // the comparisons that order them shared out among the threads).
   // Every CTA then reads all lengths, so not where the first ones to finish overwrite them.
   const int64_t lens_bytes = static_cast<int64_t>(c->batch) * (c->lens_dtype == AKL_IDX_I64 ? 8 : 4);
   const int64_t apart = static_cast<const char*>(c->kv_lens_out) - static_cast<const char*>(c->kv_lens);

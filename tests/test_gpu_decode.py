@@ -512,6 +512,28 @@ def test_eviction_of_long_rows_in_a_graph(pkg, cuda):
         assert counts.tolist() == [0, 0]
 
 
+def test_eviction_of_a_row_named_again_stays_in_bounds(pkg, cuda):
+    """Distinct rows are the caller's part; where two requests change one row at once, longer than shared
+    memory holds, its result is anybody's, but nothing outside it and the requests' own entries is written."""
+    batch, width, keep = 80, 40000, 3000
+    g = torch.Generator().manual_seed(61)
+    table = torch.randint(0, 1 << 30, (3, width + 64), generator=g, dtype=I32).to(cuda)
+    w = torch.rand((3, width + 64), generator=g).to(cuda)
+    kept = table.clone(), w.clone()
+    rows, lens = torch.ones(batch, dtype=I32, device=cuda), torch.full((batch,), width, dtype=I32, device=cuda)
+    freed = torch.full((batch + 2, width - keep + 8), -5, dtype=I32, device=cuda)
+    counts = torch.zeros(batch, dtype=I32, device=cuda)
+    for _ in range(3):
+        w[1] = kept[1][1]
+        lens.fill_(width)
+        pkg.evict_lightest(table[:, :width], w[:, :width], lens, keep=keep, rows=rows, freed=freed[1:-1, :width - keep], freed_lens=counts)
+        torch.cuda.synchronize()
+        assert bool((freed[0] == -5).all()) and bool((freed[-1] == -5).all()) and bool((freed[:, width - keep:] == -5).all())
+        for got, before in zip((table, w), kept):
+            assert torch.equal(got[0], before[0]) and torch.equal(got[2], before[2]) and torch.equal(got[1, width:], before[1, width:])
+        assert bool(((lens >= 0) & (lens <= width) & (lens + counts == width)).all())
+
+
 # ---- together --------------------------------------------------------------------------------------
 def test_prefill_judge_decode_evict_decode(pkg, cuda):
     """One request's life: prefill, the prompt's weights, decode steps that go on with them, an eviction,
