@@ -248,15 +248,24 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
             _reject(f"freed shape {tuple(freed.shape)} must be at least {(batch, max(1, width - keep))}", field="freed",
                     value=tuple(freed.shape), supported=(batch, max(1, width - keep)))
         _check_table("freed", freed)
-        if _overlap(freed, page_table) or _overlap(freed, table_out):
-            _reject("freed must not overlap the page table", field="freed", value="overlaps",
-                    supported="a distinct allocation")
     if freed_lens is not None:
         _need("freed_lens", freed_lens, (torch.int32,), 1, device, "[batch]")
         _check_batch_vector("freed_lens", freed_lens, batch, device)
-        if _overlap(freed_lens, kv_lens) or _overlap(freed_lens, lens_out):
-            _reject("freed_lens must not overlap kv_lens", field="freed_lens", value="overlaps",
-                    supported="a distinct allocation")
+    others = [("page_table", page_table), ("page_table_out", table_out), ("weights", weights),
+              ("weights_out", weights_out), ("kv_lens", kv_lens), ("kv_lens_out", lens_out)]
+    if rows is not None:
+        others.append(("rows", rows))
+        if _overlap(lens_out, rows):
+            _reject("kv_lens_out must not overlap rows", field="kv_lens_out", value="overlaps",
+                    supported="kv_lens or a distinct allocation")
+    for name, t in (("freed", freed), ("freed_lens", freed_lens)):
+        if t is None:
+            continue
+        for other, u in others:
+            if _overlap(t, u):
+                _reject(f"{name} must not overlap {other}", field=name, value="overlaps",
+                        supported="a distinct allocation")
+        others.append((name, t))
 
 
 def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: int = 0, protect_last: int = 0, rows=None,
@@ -348,20 +357,26 @@ def _ordinary_evict(page_table, weights, kv_lens, keep, first, last, rows, table
             lens_out_ptr = lens_out.data_ptr()
             if 0 < abs(lens_out_ptr - lens_ptr) < lens_bytes:
                 return no
-        for at in (table_ptr, table_out_ptr):
-            if freed_ptr < at + table_bytes and at < freed_ptr + batch * freed_width * item:
-                return no
-        for at in (lens_ptr, lens_out_ptr):
-            if count_ptr < at + lens_bytes and at < count_ptr + batch * 4:
-                return no
-        rows_ptr = rows_type = 0
+        rows_ptr = rows_type = rows_bytes = 0
         if rows is not None:
             rows_type = _INDEX[rows.dtype]
             if rows.shape != (batch,) or not rows.is_contiguous() or rows.get_device() != index:
                 return no
             rows_ptr = rows.data_ptr()
+            rows_bytes = batch * (8 if rows_type == 0 else 4)
+            if lens_out_ptr < rows_ptr + rows_bytes and rows_ptr < lens_out_ptr + lens_bytes:
+                return no
         elif table_rows < batch:
             return no
+        freed_end, count_end = freed_ptr + batch * freed_width * item, count_ptr + batch * 4
+        if freed_ptr < count_end and count_ptr < freed_end:
+            return no
+        for at, end in ((table_ptr, table_ptr + table_bytes), (table_out_ptr, table_out_ptr + table_bytes),
+                        (weights_ptr, weights_ptr + acc_bytes), (acc_out_ptr, acc_out_ptr + acc_bytes),
+                        (lens_ptr, lens_ptr + lens_bytes), (lens_out_ptr, lens_out_ptr + lens_bytes),
+                        (rows_ptr, rows_ptr + rows_bytes)):
+            if freed_ptr < end and at < freed_end or count_ptr < end and at < count_end:
+                return no
     except (AttributeError, TypeError, ValueError, KeyError):
         return no
     return index, kernel.pack_evict(table_ptr, weights_ptr, rows_ptr, lens_ptr, table_out_ptr, acc_out_ptr, lens_out_ptr,

@@ -237,6 +237,37 @@ def test_short_extend_leaves_refusals_to_the_full_form(pkg, short, field, over):
     assert e.value.field == field and not short[2]
 
 
+_SHARED = [("freed", "rows"), ("freed", "kv_lens"), ("freed", "weights"), ("freed", "weights_out"), ("freed", "page_table_out"),
+           ("freed_lens", "freed"), ("freed_lens", "rows"), ("freed_lens", "page_table"), ("freed_lens", "weights_out"),
+           ("freed_lens", "kv_lens_out"), ("kv_lens_out", "rows")]
+
+
+@pytest.mark.parametrize("quick", [False, True])
+@pytest.mark.parametrize("field,other", _SHARED)
+def test_eviction_outputs_share_no_memory(pkg, short, field, other, quick, monkeypatch):
+    """Refused wherever the shared entry lies; the same tensors one entry apart are taken."""
+    _, eviction, seen = short
+    if not quick:
+        monkeypatch.setattr(eviction, "_ordinary_evict", lambda *a: (None, None))
+    shapes = dict(freed=(2, 6), freed_lens=(2,), rows=(2,), kv_lens=(2,), kv_lens_out=(2,), page_table=(4, 12),
+                  page_table_out=(4, 12), weights=(4, 12), weights_out=(4, 12))
+    size = {k: torch.Size(v).numel() for k, v in shapes.items()}
+    for at, refused in ((0, True), (size[other] - 1, True), (size[other], False)):
+        buf = torch.zeros(size[other] + size[field], dtype=torch.int32)
+        kw = {k: torch.zeros(v, dtype=torch.float32 if k.startswith("weights") else torch.int32)
+              for k, v in shapes.items()}
+        kw[field] = buf[at:at + size[field]].view(shapes[field])
+        kw[other] = buf[:size[other]].view(kw[other].dtype).view(shapes[other])
+        kw.update(keep=8)
+        if refused:
+            with pytest.raises(pkg.CapabilityError) as e:
+                pkg.evict_lightest(**kw)
+            assert e.value.field == field and not seen
+        else:
+            pkg.evict_lightest(**kw)
+            assert len(seen) == 1
+
+
 @pytest.mark.parametrize("field,over", EVICT_REFUSALS, ids=_IDS)
 def test_short_eviction_leaves_refusals_to_the_full_form(pkg, short, field, over):
     base = dict(_evict(weights=torch.zeros(4, 12)), freed=torch.zeros(2, 6, dtype=torch.int32),
