@@ -373,8 +373,8 @@ def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, we
             return None
         index = ws.device_index
         max_requests, q_heads, kv_heads, _, max_tokens = ws._plan_fields
-        batch, heads, dim = q.shape
-        pool_shape = k_pool.shape
+        q_shape, pool_shape = q.shape, k_pool.shape
+        batch, heads, dim = q_shape
         pool, kv, kv_dim = pool_shape
         table_shape = page_table.shape
         table_rows, width = table_shape
@@ -382,7 +382,7 @@ def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, we
         if (index < 0 or heads != q_heads or kv != kv_heads or dim != 256 or kv_dim != 256
                 or not 1 <= batch <= max_requests or not 1 <= pool < 1 << 31 or not 1 <= table_rows < 1 << 31
                 or not 1 <= width < 1 << 31 or v_pool.shape != pool_shape or v_pool.dtype is not k_pool.dtype
-                or q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q.shape
+                or q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q_shape
                 or kv_lens.shape != (batch,)
                 or not (q.is_contiguous() and k_pool.is_contiguous() and v_pool.is_contiguous()
                         and page_table.is_contiguous() and kv_lens.is_contiguous() and out.is_contiguous())
