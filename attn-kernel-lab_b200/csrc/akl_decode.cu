@@ -21,11 +21,11 @@
 //     be padding.  Out^T = V^T P^T takes P^T in the operand layout that an 8x8 transpose of the score
 //     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: a tile needs 8192
 //     multiply-adds per position and kv head against the ~43 cycles that its bytes take per SM (the tensor
-//     pipe is 15 to 19 % busy); tcgen05's 128 rows would be 6 to 25 % filled and its TMEM round trip longer.
+//     pipe is 9 to 13 % busy); tcgen05's 128 rows would be 6 to 25 % filled and its TMEM round trip longer.
 //
-// Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 360 to 369 us, 92 to 95 % of the
-// copy bandwidth; one request of 139264 positions, 571 MB, 102 to 111 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
-// 8.8 us.  The short ones are bound by three dependent trips to memory (lengths, page table, rows) and the join,
+// Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 364 to 368 us, 92 to 93 % of the
+// copy bandwidth; one request of 139264 positions, 571 MB, 104 to 109 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
+// 8.7 us.  The short ones are bound by three dependent trips to memory (lengths, page table, rows) and the join,
 // the long ones by HBM and by the SMs that get their equal share up to 8 % later than the median.
 //
 // Rounding: scores, m, l and both sums are 32-bit.  P enters the second product as two 16-bit parts,

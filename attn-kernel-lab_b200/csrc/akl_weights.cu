@@ -18,9 +18,9 @@
 // in it.  A CTA's first piece may continue the one of the CTA before it and then goes to a place of its own; the last launch
 // adds the pieces of a position in a fixed order.
 //
-// Measured (a call in a CUDA graph, 24:4 heads): 2048 rows over 10240 positions 172 us, 1350 TFLOP/s of the
+// Measured (a call in a CUDA graph, 24:4 heads): 2048 rows over 10240 positions 172 to 174 us, 1340 TFLOP/s of the
 // product; tensor pipe and exponential unit 75 % busy in the main launch, the packing in front of it 8 us.  32 rows
-// over 4097: 12.6 us, the latency of three launches.
+// over 4097: 12.7 us, the latency of three launches.
 //
 // Rounding: scores and sums are 32-bit.  BF16 queries meet a BF16 pool unchanged; for an FP16 pool
 // a row is divided by the power of two of its largest element and rounded to FP16: exact down to
