@@ -1,0 +1,39 @@
+"""Decode attention where its sums, masks and limits can go wrong."""
+import math
+
+import pytest
+import torch
+
+import decode_ref as R
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, I32, I64 = torch.bfloat16, torch.float16, torch.int32, torch.int64
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_decode_sums_over_positions_are_rounded_not_truncated(pkg, cuda, dtype):
+    """Position n and position n + half have one key and opposite values, so every output is exactly 0 and
+    what comes out is what the sum over the positions lost on its way up and down again.
+
+    With a request per SM a warp adds `tiles` = 2 half / 16 tile sums, one rounding each: off by at most
+    half a step of the running sum |o| <= l / 2 (values are at most 1, and the two halves weigh l / 2), of
+    standard deviation step / sqrt(12) with a step of 2^-23 |o| at most.  Six standard deviations of
+    `tiles` of them, divided by l, are the bound.  Tile sums themselves cancel: equal probabilities (the largest
+    score comes first, so no maximum moves later) and mirrored values, in the same places of their tiles.
+    A sum that is cut off at 32 bits twice a tile loses 2 tiles x 0.36 steps of l / 4 x 0.75, three to five bounds."""
+    half, heads, kv = 8192, 24, 4
+    batch = torch.cuda.get_device_properties(cuda).multi_processor_count
+    g = torch.Generator().manual_seed(1)
+    k = torch.randn((half, kv, 256), generator=g)
+    k[:, :, 0] = 0.0
+    k[0, :, 0] = 8.0
+    v = torch.rand((half, kv, 256), generator=g) * 0.5 + 0.5
+    q = torch.randn((batch, heads, 256), generator=g) * 0.5
+    q[:, :, 0] = 8.0                                             # scores of +-0.7, and 5.8 more for the first key
+    pool = dict(k_pool=torch.cat([k, k]).to(dtype).to(cuda), v_pool=torch.cat([v, -v]).to(dtype).to(cuda))
+    out = pkg.paged_decode(q.to(BF16).to(cuda), **pool, page_table=torch.arange(2 * half, device=cuda)[None],
+                           kv_lens=torch.full((batch,), 2 * half, device=cuda), rows=torch.zeros(batch, dtype=I32, device=cuda))
+    bound = 6 * math.sqrt(2 * half / 16) * 2.0 ** -23 / math.sqrt(12) / 2
+    worst = float(out.float().abs().max())
+    assert worst <= bound, f"{worst:.3g}, bound {bound:.3g}"
