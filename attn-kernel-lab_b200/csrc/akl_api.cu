@@ -70,7 +70,7 @@ int build_geom(const akl_call_t* c, Geom* g) {
   if (c->q_heads < 1 || c->kv_heads < 1 || c->q_heads % c->kv_heads) return AKL_ERR_UNSUPPORTED;
   if (c->kv_pos0 < 0 || c->kv_pos0 % kTile) return AKL_ERR_INVALID;
   if (!(c->sm_scale > 0.f)) return AKL_ERR_INVALID;
-  if (c->flags & ~(AKL_FLAG_ROTATE | AKL_FLAG_CENTER_K | AKL_FLAG_QK_I8)) return AKL_ERR_INVALID;   // unknown mode bit
+  if (c->flags & ~(AKL_FLAG_ROTATE | AKL_FLAG_CENTER_K | AKL_FLAG_QK_I8 | AKL_FLAG_POOL_LSE)) return AKL_ERR_INVALID;   // unknown mode bit
   akl_ws_layout_t L;
   int rc = compute_layout(c->plan, &L);
   if (rc != AKL_OK) return rc;
@@ -194,7 +194,7 @@ int check_batch(const akl_batch_t* b, BatchLayout* L) {
   if (b->kv_dtype != AKL_KV_BF16 && b->kv_dtype != AKL_KV_FP16) return AKL_ERR_INVALID;
   if (b->idx_dtype != AKL_IDX_I64 && b->idx_dtype != AKL_IDX_I32) return AKL_ERR_INVALID;
   if (!(b->sm_scale > 0.f)) return AKL_ERR_INVALID;
-  if (b->flags & ~(AKL_FLAG_ROTATE | AKL_FLAG_CENTER_K | AKL_FLAG_QK_I8)) return AKL_ERR_INVALID;
+  if (b->flags & ~(AKL_FLAG_ROTATE | AKL_FLAG_CENTER_K | AKL_FLAG_QK_I8 | AKL_FLAG_POOL_LSE)) return AKL_ERR_INVALID;
   int rc = compute_batch_layout(b->caps, L);
   if (rc != AKL_OK) return rc;
   if (b->workspace_bytes < L->ws_bytes || b->table_bytes < L->table_bytes) return AKL_ERR_CAPACITY;
@@ -315,7 +315,9 @@ int akl_attention(const akl_call_t* c, void* stream) {
   int rc = build_geom(c, &g);
   if (rc != AKL_OK) return rc;
   if ((rc = need_out(c)) != AKL_OK) return rc;
-  return launch_attention(g, static_cast<cudaStream_t>(stream));
+  if ((g.flags & AKL_FLAG_POOL_LSE) && (rc = need_q(c)) != AKL_OK) return rc;
+  if ((rc = launch_attention(g, static_cast<cudaStream_t>(stream))) != AKL_OK) return rc;
+  return launch_pool_lse(g, static_cast<cudaStream_t>(stream));
 }
 
 int akl_attention_dump(const akl_call_t* c, float* s_dump, uint8_t* p_dump, void* stream) {
@@ -326,7 +328,9 @@ int akl_attention_dump(const akl_call_t* c, float* s_dump, uint8_t* p_dump, void
   if (s_dump == nullptr || p_dump == nullptr) return AKL_ERR_INVALID;
   g.dbg_s = s_dump;
   g.dbg_p = p_dump;
-  return launch_attention(g, static_cast<cudaStream_t>(stream), true);
+  if ((g.flags & AKL_FLAG_POOL_LSE) && (rc = need_q(c)) != AKL_OK) return rc;
+  if ((rc = launch_attention(g, static_cast<cudaStream_t>(stream), true)) != AKL_OK) return rc;
+  return launch_pool_lse(g, static_cast<cudaStream_t>(stream));
 }
 
 int akl_prefill_extend(const akl_call_t* c, void* stream) {
@@ -337,7 +341,8 @@ int akl_prefill_extend(const akl_call_t* c, void* stream) {
   if ((rc = launch_kv_tile_stats(g, c->kv_dtype, c->idx_dtype, s, /*with_q=*/true)) != AKL_OK) return rc;
   if ((rc = launch_kv_means(g, s, /*fuse_scales=*/true)) != AKL_OK) return rc;
   if ((rc = launch_kv_transform(g, c->kv_dtype, c->idx_dtype, s)) != AKL_OK) return rc;
-  return launch_attention(g, s);
+  if ((rc = launch_attention(g, s)) != AKL_OK) return rc;
+  return launch_pool_lse(g, s);
 }
 
 int akl_batch_layout(const akl_batch_caps_t* caps, akl_batch_layout_t* out) {
@@ -486,7 +491,9 @@ int akl_prefill_extend_batch_phases(const akl_batch_t* b, uint32_t phases, void*
       cudaError_t e = cudaMemsetAsync(&batch_header(ref)->attn_counter, 0, sizeof(int32_t), s);
       if (e != cudaSuccess) { note_cuda_error(e, "cudaMemsetAsync(work counter)"); return AKL_ERR_CUDA; }
     }
-    return launch_batch_attention(ref, (b->flags & AKL_FLAG_QK_I8) != 0, sms, s);
+    if ((rc = launch_batch_attention(ref, (b->flags & AKL_FLAG_QK_I8) != 0, sms, s)) != AKL_OK) return rc;
+    constexpr uint32_t kAdds = AKL_FLAG_POOL_LSE | AKL_FLAG_CENTER_K;
+    if ((b->flags & kAdds) == kAdds) return launch_batch_pool_lse(ref, sms, s);
   }
   return AKL_OK;
 }

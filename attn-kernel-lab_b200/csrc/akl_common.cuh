@@ -360,11 +360,13 @@ int launch_kv_transform(const Geom& g, int kv_dtype, int idx_dtype, cudaStream_t
 int launch_quantize_q(const Geom& g, cudaStream_t s);
 int launch_attention(const Geom& g, cudaStream_t s, bool dump = false);
 int launch_merge(const akl_merge_t& m, cudaStream_t s);
+int launch_pool_lse(const Geom& g, cudaStream_t s);
 // batched forms: every kernel reads counts and per-request geometry from the request table
 int launch_batch_stats(const BatchRef& b, int kv_dtype, int idx_dtype, int sm_count, cudaStream_t s);
 int launch_batch_means(const BatchRef& b, int kv_heads, cudaStream_t s);
 int launch_batch_transform(const BatchRef& b, int kv_dtype, int idx_dtype, int sm_count, cudaStream_t s);
 int launch_batch_attention(const BatchRef& b, bool qk_i8, int sm_count, cudaStream_t s);
+int launch_batch_pool_lse(const BatchRef& b, int sm_count, cudaStream_t s);
 int launch_exact_division_selftest(const float* scales, int n, unsigned long long* mismatches, cudaStream_t s);
 int device_sm_count(int* out);
 void note_cuda_error(cudaError_t e, const char* where);

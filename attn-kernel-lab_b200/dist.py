@@ -116,7 +116,8 @@ def row_slices(rows: int, world: int):
 
 # ------------------------------------------------------------------ merge (single device)
 def merge_states(parts_o, parts_lse, out=None, lse_out=None):
-    """Merge per-split partial states with the `akl_merge_states` kernel.
+    """Merge per-split partial states with the `akl_merge_states` kernel.  Their LSEs must be of one set of
+    scores: a state of `paged_decode` goes with states of `prefill_extend(..., pool_lse=True)`.
 
     parts_o: list of [rows, 256] (or [T, H, 256]) BF16 tensors on one device; parts_lse: list of
     matching FP32 base-2 LSE tensors.  Returns (out, lse)."""
@@ -143,11 +144,12 @@ def merge_states(parts_o, parts_lse, out=None, lse_out=None):
 # ------------------------------------------------------------------ KV-axis split of one request
 def kv_split_local(ws, q, k_pool, v_pool, idx_local, prefix: int, *, n_total: int, kv_lo: int,
                    sm_scale: float, rotate: bool = True, center_k: bool = True, qk_i8: bool = False,
-                   all_reduce_sum=None, all_reduce_max=None, phases=None):
+                   all_reduce_sum=None, all_reduce_max=None, phases=None, pool_lse: bool = False):
     """One rank's share of a KV-split request: statistics made global through the two
     callbacks, then transform + attention over local positions [kv_lo, kv_lo + len(idx_local)).
 
-    Returns (O_i [T, Hq, 256] BF16 normalised with the V mean added, lse_i [T, Hq] FP32).
+    Returns (O_i [T, Hq, 256] BF16 normalised with the V mean added, lse_i [T, Hq] FP32; with `pool_lse`
+    over the pool's own keys, as in `prefill_extend` -- the mean is global, so either form merges).
     `all_reduce_sum(t)` / `all_reduce_max(t)` reduce a tensor in place across ranks (identity
     for a single-rank emulation that shares the arrays).  `phases(name, call)` runs one phase
     entry point; the default calls the native library on the current stream (host-logic tests
@@ -173,7 +175,7 @@ def kv_split_local(ws, q, k_pool, v_pool, idx_local, prefix: int, *, n_total: in
         ws, q=q, k_pool=k_pool, v_pool=v_pool, idx=idx_local, out=out, lse_out=lse, q_len=T,
         kv_len=max(n_local, 1), prefix=prefix, q_heads=Hq, kv_heads=Hkv, sm_scale=sm_scale,
         rotate=rotate, center_k=center_k, qk_i8=qk_i8, kv_pos0=kv_lo, n_total=n_total,
-        tile0_global=kv_lo // _quant.BLK, ntiles_global=ntg)
+        tile0_global=kv_lo // _quant.BLK, ntiles_global=ntg, pool_lse=pool_lse)
     ktsum, vtsum = ws.view("ktsum"), ws.view("vtsum")
     ktsum[:ntg].zero_()
     vtsum[:ntg].zero_()
@@ -199,7 +201,8 @@ def kv_split_local(ws, q, k_pool, v_pool, idx_local, prefix: int, *, n_total: in
 
 def prefill_extend_kv_split(ws, q, k_pool, v_pool, idx_local, prefix: int, *, n_total: int,
                             kv_lo: int, sm_scale: float, group=None, rotate: bool = True,
-                            center_k: bool = True, qk_i8: bool = False, phases=None, merge=None):
+                            center_k: bool = True, qk_i8: bool = False, phases=None, merge=None,
+                            pool_lse: bool = False):
     """KV-axis split of one long request across the ranks of `group` (default: world).
 
     Every rank passes the full `q`, its own slice of the page table (`idx_local`, global
@@ -219,7 +222,8 @@ def prefill_extend_kv_split(ws, q, k_pool, v_pool, idx_local, prefix: int, *, n_
 
     o_i, lse_i = kv_split_local(ws, q, k_pool, v_pool, idx_local, prefix, n_total=n_total,
                                 kv_lo=kv_lo, sm_scale=sm_scale, rotate=rotate, center_k=center_k,
-                                qk_i8=qk_i8, all_reduce_sum=ar_sum, all_reduce_max=ar_max, phases=phases)
+                                qk_i8=qk_i8, all_reduce_sum=ar_sum, all_reduce_max=ar_max, phases=phases,
+                                pool_lse=pool_lse)
     return exchange_and_merge(o_i, lse_i, group=group, merge=merge)
 
 

@@ -1,7 +1,7 @@
 """Bounding a request's cache by what its tokens were attended to.
 
 `extend_weights` adds up what the query rows of an extend (all of them, or the last ones as a window)
-put on every cached position, from the log-sum-exp that `prefill_extend` returns; `paged_decode` with
+put on every cached position, from the log-sum-exp that `prefill_extend` returns with `pool_lse`; `paged_decode` with
 `weights` goes on with the same accumulator token by token.  `evict_lightest` then shortens page-table
 rows to the heaviest positions, in place, and lists the slots that became free.  The pool itself is
 never moved: a slot is a page.
@@ -106,8 +106,9 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
 
     `q` [q_len, q_heads, 256] BF16, `k_pool` [pool, kv_heads, 256] BF16 or FP16, `idx` [kv_len] int32 or
     int64 and `prefix` as in `prefill_extend`: row t sees the positions 0 .. prefix + t.  `lse` [q_len,
-    q_heads] FP32 base 2 is what that call returned (of any softmax over the same scores).  `weights`
-    [kv_len] FP32 becomes `weight_decay` times itself plus
+    q_heads] FP32 base 2 is the log-sum-exp of the scores of the pool's own keys: what that call returned
+    with `pool_lse=True` (or with `center_k=False`; the default's is over centred keys, and would put every row
+    off by a factor of its own).  `weights` [kv_len] FP32 becomes `weight_decay` times itself plus
 
         sum over t, h with i <= prefix + t of 2^(sm_scale log2e <q[t, h], k_i> - lse[t, h]).
 

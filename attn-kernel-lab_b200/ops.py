@@ -253,7 +253,7 @@ def plan_workspace(device, *, max_kv_len: int, max_q_len: int, q_heads: int | No
 def prefill_extend(q, k_pool, v_pool, idx, prefix, *, workspace=None, out=None, lse_out=None,
                    sm_scale=None, qk_i8: bool = True, rotate: bool = True, center_k: bool = True,
                    return_lse: bool = False, capability: OperatorCapability = V1_CAPABILITY,
-                   check_status: bool = False):
+                   check_status: bool = False, pool_lse: bool = False):
     """Bottom-right-causal paged EXTEND attention over a page-size-1 BF16/FP16 KV pool.
 
     Arguments as in the reference (ops.py:485-553): `q` [q_len, q_heads, 256] BF16; `k_pool`,
@@ -265,12 +265,17 @@ def prefill_extend(q, k_pool, v_pool, idx, prefix, *, workspace=None, out=None, 
     status word and raises `NativeError(AKL_ERR_TIMEOUT)` if a bounded device-side wait ran out
     (the kernel then wrote NaN rows and +inf LSE instead of results).
 
-    Returns `out`, or `(out, lse)` with `lse` [q_len, q_heads] FP32 base-2 when `return_lse`."""
+    Returns `out`, or `(out, lse)` with `lse` [q_len, q_heads] FP32 base-2 when `return_lse`.  As in the
+    reference, that is the log-sum-exp over the keys as they were quantised: with `center_k` over the
+    centred ones, which is smaller by sm_scale log2e <q, mean of the request's keys>.  `pool_lse` (not in
+    the reference; one more short launch) adds that term: the LSE over the pool's own keys, as
+    `extend_weights` needs it and as it can be merged with the LSE of `paged_decode`."""
     request = check_request(q, k_pool, v_pool, idx, prefix, workspace=workspace, out=out,
                             lse_out=lse_out, sm_scale=sm_scale, return_lse=return_lse,
                             capability=capability)
     if not isinstance(qk_i8, bool):
         raise TypeError(f"qk_i8 must be a bool, got {type(qk_i8).__name__}")
+    _check_pool_lse(pool_lse, return_lse)
 
     # ---- everything below touches the device -------------------------------------------
     import torch
@@ -294,13 +299,21 @@ def prefill_extend(q, k_pool, v_pool, idx, prefix, *, workspace=None, out=None, 
         ws, q=q, k_pool=k_pool, v_pool=v_pool, idx=idx, out=out, lse_out=lse,
         q_len=request.q_len, kv_len=request.kv_len, prefix=request.prefix,
         q_heads=request.q_heads, kv_heads=request.kv_heads, sm_scale=request.sm_scale,
-        rotate=rotate, center_k=center_k, qk_i8=qk_i8)
+        rotate=rotate, center_k=center_k, qk_i8=qk_i8, pool_lse=pool_lse)
     with torch.cuda.device(q.device):
         code = lib.akl_prefill_extend(ctypes.byref(call), torch.cuda.current_stream(q.device).cuda_stream)
     kernel_mod.check(code, "akl_prefill_extend")
     if check_status:
         _raise_on_status(ws, kernel_mod, "akl_prefill_extend")
     return (out, lse) if request.return_lse else out
+
+
+def _check_pool_lse(pool_lse, return_lse) -> None:
+    if not isinstance(pool_lse, bool):
+        raise TypeError(f"pool_lse must be a bool, got {type(pool_lse).__name__}")
+    if pool_lse and not return_lse:
+        _reject("pool_lse=True but return_lse=False: a form of an output that will not be produced is a caller "
+                "mistake", field="pool_lse", value=True, supported="return_lse=True")
 
 
 def _raise_on_status(ws, kernel_mod, where: str) -> None:
@@ -330,7 +343,7 @@ def plan_batch_workspace(device, *, max_requests: int, max_total_kv_len: int, ma
                                     max_total_q_len=max_total_q_len, q_heads=q_heads, kv_heads=kv_heads)
 
 
-def _native_batch(requests, ws, *, sm_scale, qk_i8, rotate, center_k, return_lse, capability):
+def _native_batch(requests, ws, *, sm_scale, qk_i8, rotate, center_k, return_lse, capability, pool_lse):
     """Validate every request, give the ones without `out` / `lse_out` their tensors, group by
     (kv dtype, idx dtype) -- one native batch per group, normally one -- and launch."""
     import torch
@@ -370,7 +383,7 @@ def _native_batch(requests, ws, *, sm_scale, qk_i8, rotate, center_k, return_lse
         groups.setdefault((r["k_pool"].dtype, r["idx"].dtype), []).append(i)
     for members in groups.values():
         plan = ws.plan([filled[i] for i in members], sm_scale=checked[members[0]].sm_scale,
-                       rotate=rotate, center_k=center_k, qk_i8=qk_i8)
+                       rotate=rotate, center_k=center_k, qk_i8=qk_i8, pool_lse=pool_lse)
         ws.launch(plan)
     return [(d["out"], d["lse_out"]) if c.return_lse else d["out"] for d, c in zip(filled, checked)]
 
@@ -391,7 +404,7 @@ def _streams_for(device, count: int):
 
 def prefill_extend_batch(requests, *, workspace, sm_scale=None, qk_i8: bool = True, rotate: bool = True,
                          center_k: bool = True, return_lse: bool = False,
-                         capability: OperatorCapability = V1_CAPABILITY):
+                         capability: OperatorCapability = V1_CAPABILITY, pool_lse: bool = False):
     """Run a list of independent requests; results are exactly those of `prefill_extend` per
     request (the reference loops per request the same way,
     engines/sglang/integration/fp8_prefill/backend.py:267-289).
@@ -411,11 +424,12 @@ def prefill_extend_batch(requests, *, workspace, sm_scale=None, qk_i8: bool = Tr
     whole batch can be captured in one CUDA graph); callers see ordinary stream semantics.
     Returns the list of results in request order."""
     requests = list(requests)
+    _check_pool_lse(pool_lse, return_lse)
     from .quant import FP8PrefillBatchWorkspace
 
     if isinstance(workspace, FP8PrefillBatchWorkspace):
         return _native_batch(requests, workspace, sm_scale=sm_scale, qk_i8=qk_i8, rotate=rotate,
-                             center_k=center_k, return_lse=return_lse, capability=capability)
+                             center_k=center_k, return_lse=return_lse, capability=capability, pool_lse=pool_lse)
     pool = list(workspace) if isinstance(workspace, (list, tuple)) else [workspace]
     # longest-processing-time-first assignment of requests to workspaces / streams
     cost = [int(r["q"].shape[0]) * (int(r["prefix"]) + (int(r["q"].shape[0]) + 1) / 2.0)
@@ -449,7 +463,7 @@ def prefill_extend_batch(requests, *, workspace, sm_scale=None, qk_i8: bool = Tr
         return prefill_extend(r["q"], r["k_pool"], r["v_pool"], r["idx"], r["prefix"], workspace=ws,
                               out=r.get("out"), lse_out=r.get("lse_out"), sm_scale=sm_scale,
                               qk_i8=qk_i8, rotate=rotate, center_k=center_k, return_lse=return_lse,
-                              capability=capability)
+                              capability=capability, pool_lse=pool_lse)
 
     if len(pool) == 1 or not requests:
         return [run(r, pool[0]) for r in requests]

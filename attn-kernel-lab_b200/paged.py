@@ -23,13 +23,14 @@ def _is_tensor(x) -> bool:
 
 def fp8_paged_prefill(q, paged_k_cache, paged_v_cache, kv_indices, *, page_size: int = 1,
                       causal: bool = True, sm_scale=None, out=None, return_lse: bool = False,
-                      workspace_buffer=None, capability: OperatorCapability = V1_CAPABILITY):
+                      workspace_buffer=None, capability: OperatorCapability = V1_CAPABILITY,
+                      pool_lse: bool = False):
     """Returns `out` [qo_len, num_qo_heads, 256] BF16 (the caller's `out` when given), or
     `(out, lse)` with base-2 `lse` [qo_len, num_qo_heads] FP32 when `return_lse`.
 
     `workspace_buffer` is an `FP8PrefillWorkspace` (named after the upstream argument); with a
     planned workspace the call allocates nothing but `out`.  Everything else -- validation order,
-    error types, stream semantics -- is `prefill_extend`'s."""
+    error types, stream semantics, which keys the LSE is over (`pool_lse`) -- is `prefill_extend`'s."""
     if not _is_tensor(q) or q.dim() != 3:
         raise ValueError("q must be a 3-D [qo_len, num_qo_heads, head_dim] tensor")
     for name, cache in (("paged_k_cache", paged_k_cache), ("paged_v_cache", paged_v_cache)):
@@ -57,4 +58,5 @@ def fp8_paged_prefill(q, paged_k_cache, paged_v_cache, kv_indices, *, page_size:
     v_pool = paged_v_cache[:, 0]
     prefix = int(kv_indices.numel()) - int(q.shape[0])
     return ops.prefill_extend(q, k_pool, v_pool, kv_indices, prefix, workspace=workspace_buffer,
-                              out=out, sm_scale=sm_scale, return_lse=return_lse, capability=capability)
+                              out=out, sm_scale=sm_scale, return_lse=return_lse, capability=capability,
+                              pool_lse=pool_lse)

@@ -344,14 +344,14 @@ class FP8PrefillBatchWorkspace:
         _kernel.check(code, "akl_batch_plan")
 
     def plan(self, requests, *, sm_scale: float, rotate: bool = True, center_k: bool = True,
-             qk_i8: bool = False) -> BatchPlan:
+             qk_i8: bool = False, pool_lse: bool = False) -> BatchPlan:
         """Host-side only: pack `requests` (dicts with q, k_pool, v_pool, idx, prefix, out and
         optionally lse_out; one kv dtype and one idx dtype) into a fresh pinned request table."""
         requests = list(requests)
         if not requests:
             raise ValueError("an empty batch has nothing to plan")
         flags = ((_kernel.AKL_FLAG_ROTATE if rotate else 0) | (_kernel.AKL_FLAG_CENTER_K if center_k else 0)
-                 | (_kernel.AKL_FLAG_QK_I8 if qk_i8 else 0))
+                 | (_kernel.AKL_FLAG_QK_I8 if qk_i8 else 0) | (_kernel.AKL_FLAG_POOL_LSE if pool_lse else 0))
         batch = self._batch_struct(_dtype_code(requests[0]["k_pool"]), _idx_code(requests[0]["idx"]), flags, sm_scale)
         pin = self.device.type == "cuda"
         table_host = torch.empty(self._table_bytes, dtype=torch.uint8, pin_memory=pin)
@@ -410,7 +410,8 @@ def _idx_code(t: torch.Tensor) -> int:
 def make_call(ws: FP8PrefillWorkspace, *, q=None, k_pool, v_pool, idx, out=None, lse_out=None,
               q_len: int, kv_len: int, prefix: int, q_heads: int, kv_heads: int, sm_scale: float,
               rotate: bool = True, center_k: bool = True, qk_i8: bool = False, kv_pos0: int = 0,
-              n_total: int = 0, tile0_global: int = 0, ntiles_global: int = 0) -> "_kernel.Call":
+              n_total: int = 0, tile0_global: int = 0, ntiles_global: int = 0,
+              pool_lse: bool = False) -> "_kernel.Call":
     """Fill an `akl_call_t` from tensors (pointers only; nothing is copied or launched)."""
     mk, mq, hq, hkv = ws.dims
     c = _kernel.Call()
@@ -428,7 +429,7 @@ def make_call(ws: FP8PrefillWorkspace, *, q=None, k_pool, v_pool, idx, out=None,
     c.kv_dtype = _dtype_code(k_pool)
     c.idx_dtype = _idx_code(idx) if idx.dtype in (torch.int64, torch.int32) else _kernel.AKL_IDX_I64
     c.flags = ((_kernel.AKL_FLAG_ROTATE if rotate else 0) | (_kernel.AKL_FLAG_CENTER_K if center_k else 0)
-               | (_kernel.AKL_FLAG_QK_I8 if qk_i8 else 0))
+               | (_kernel.AKL_FLAG_QK_I8 if qk_i8 else 0) | (_kernel.AKL_FLAG_POOL_LSE if pool_lse else 0))
     c.sm_scale = float(sm_scale)
     c.kv_pos0, c.n_total = kv_pos0, n_total
     c.tile0_global, c.ntiles_global = tile0_global, ntiles_global

@@ -51,6 +51,11 @@ enum { AKL_IDX_I64 = 0, AKL_IDX_I32 = 1 };
 #define AKL_FLAG_CENTER_K 2u  /* subtract the K channel mean (reference kwarg center_k, ops.py:498) */
 #define AKL_FLAG_QK_I8 4u     /* Q and K as INT8 at amax/127 with an exact s32 QK^T (reference kwarg qk_i8,
                                * its default, ops.py:496; quant.py:416-430, 471-478); clear = FP8 E4M3 QK */
+/* lse_out is the log-sum-exp of the scores of the pool's keys as they are.  Without it, as in the reference, it is that
+ * of the centred keys when AKL_FLAG_CENTER_K is set: smaller by sm_scale log2e <q, kmean>, which the softmax does not
+ * notice but whoever compares or combines the LSE with scores of the pool does (akl_extend_weights, akl_paged_decode's
+ * LSE in akl_merge_states).  One more launch, which adds that term; `out` is the same. */
+#define AKL_FLAG_POOL_LSE 32u
 
 /* Capacity plan: the maxima a workspace is laid out for.
  * Replaces quant.FP8PrefillWorkspace.reserve / CapacityPlan (quant.py:175-196, :253-336). */
@@ -97,7 +102,7 @@ typedef struct akl_call {
   const void* v_pool;
   const void* idx;      /* [N] i64 | i32 pool rows in position order (values unchecked) */
   void* out;            /* [T][Hq][256] bf16 */
-  float* lse_out;       /* [T][Hq] f32 base-2 log-sum-exp, or NULL */
+  float* lse_out;       /* [T][Hq] f32 base-2 log-sum-exp (AKL_FLAG_POOL_LSE: of which keys), or NULL */
   void* workspace;      /* base of the allocation described by `plan` */
   uint64_t workspace_bytes;
   akl_plan_t plan;      /* what the workspace was laid out for */
@@ -120,7 +125,8 @@ typedef struct akl_call {
 } akl_call_t;
 
 /* (O, lse2) partial-state merge for a KV-axis split: out = sum_i 2^(lse_i - lse) O_i,
- * lse = log2 sum_i 2^lse_i.  New: the reference exposes base-2 LSE for this purpose
+ * lse = log2 sum_i 2^lse_i.  The parts' LSEs are of one set of scores: a part of akl_paged_decode goes with parts of
+ * akl_prefill_extend that have AKL_FLAG_POOL_LSE.  New: the reference exposes base-2 LSE for this purpose
  * (docs/OPERATOR_CONTRACT.md:57,238-242) but ships no merge. */
 typedef struct akl_merge {
   const void* const* parts_o;     /* device array of nparts pointers to [rows][256] bf16 */
@@ -336,7 +342,9 @@ int akl_paged_decode(const akl_decode_t* call, void* stream);
 /* ---- attention weights of an extend ----------------------------------------------------------
  * What the T query rows of an extend (or its last T rows) attend to, summed over rows and q heads:
  *   weights[i] = decay weights[i] + sum_{t, h: i <= prefix + t} 2^(sm_scale log2e <q[t][h], K[idx[i]][h / group]> - lse[t][h])
- * lse is what akl_prefill_extend writes (base 2); a row whose lse is -inf or +inf adds nothing.
+ * lse is the base-2 log-sum-exp of these same scores: what akl_prefill_extend writes with AKL_FLAG_POOL_LSE, or without
+ * AKL_FLAG_CENTER_K (with centred keys and no AKL_FLAG_POOL_LSE it is another number, and the weights are off by
+ * 2^(sm_scale log2e <q, kmean>), row by row); a row whose lse is -inf or +inf adds nothing.
  * No counterpart in the reference. */
 typedef struct akl_weights_plan {
   int32_t max_kv_len, max_q_len, q_heads, kv_heads;
