@@ -816,13 +816,13 @@ __device__ __forceinline__ void add_weights(const akl_decode_t& c, const Work& w
   long long chunk0 = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) chunk0 += sm_chunks[i];
+  if (chunk0 + (n + kChunk - 1) / kChunk > w.max_chunks) {
+    // not all of the request's scores were recorded: its row stays as it was, from the first position to the last
+    if (tid == 0) atomicCAS(w.status, 0, AKL_ERR_CAPACITY);
+    return;
+  }
   for (int i = part * 256 + tid; i < n; i += blocks * 256) {
-    const long long chunk = chunk0 + i / kChunk;
-    if (chunk >= w.max_chunks) {
-      atomicCAS(w.status, 0, AKL_ERR_CAPACITY);
-      break;
-    }
-    const float* x = w.scores + chunk * c.q_heads * kChunk + i % kChunk;
+    const float* x = w.scores + (chunk0 + i / kChunk) * c.q_heads * kChunk + i % kChunk;
     float total = 0.f;
 #pragma unroll 8
     for (int h = 0; h < c.q_heads; ++h) {

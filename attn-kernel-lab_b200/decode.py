@@ -318,8 +318,8 @@ def paged_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
     `workspace` from `plan_decode_workspace`; without one the call allocates its own (with `weights`
     sized by the table's width).  Enqueues on the current stream and does not synchronise, unless
     `check_status` (a debugging aid): then it waits and raises `NativeError` when a bounded device-side
-    wait ran out, or when the lengths exceed the plan's `max_weight_tokens` (the outputs are whole then,
-    the weights of the last requests are not).
+    wait ran out, or when the lengths exceed the plan's `max_weight_tokens` (the outputs are whole then;
+    from the first request on that does not fit, rows of `weights` are left as they were).
 
     Returns `out` [batch, q_heads, 256] BF16, or `(out, lse)` with the base-2 `lse` [batch, q_heads]."""
     if workspace is not None and out is not None and capability is DECODE_CAPABILITY:

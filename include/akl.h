@@ -309,7 +309,8 @@ typedef struct akl_decode_layout {
   uint64_t total_bytes;       /* 1024-byte aligned base */
   uint64_t off_status;        /* [64] i32; word 0 = first device error code: AKL_ERR_TIMEOUT, or
                                * AKL_ERR_CAPACITY when the lengths exceed max_weight_tokens (out and
-                               * lse are whole then, weights of the last requests are not updated) */
+                               * lse are whole then, and so are the weights of the first requests; from the
+                               * one that does not fit on, rows of weights are left as they were) */
   uint64_t off_parts;         /* partial states of requests that several CTAs share */
   uint64_t off_lse;           /* [max_requests][Hq] f32 */
   uint64_t off_scores;        /* x, f32, by 64-position chunk of the packed requests: [chunk][Hq][64] */

@@ -37,3 +37,21 @@ def test_decode_sums_over_positions_are_rounded_not_truncated(pkg, cuda, dtype):
     bound = 6 * math.sqrt(2 * half / 16) * 2.0 ** -23 / math.sqrt(12) / 2
     worst = float(out.float().abs().max())
     assert worst <= bound, f"{worst:.3g}, bound {bound:.3g}"
+
+
+@pytest.mark.parametrize("tokens,fit", [(64, 0), (128, 1), (320, 1), (384, 2), (448, 3)])
+def test_weights_beyond_the_plan_leave_whole_rows_alone(pkg, cuda, tokens, fit):
+    """A limit that falls inside a request: its row is neither decayed nor added to, in any of its places."""
+    c = R.case([100, 250, 30], 24, 4, seed=18)                   # 2, 4 and 1 chunks of 64 positions
+    ws = pkg.plan_decode_workspace(cuda, max_requests=3, q_heads=24, kv_heads=4, max_weight_tokens=tokens)
+    before = torch.rand(c["page_table"].shape, generator=torch.Generator().manual_seed(2)).to(cuda)
+    weights = before.clone()
+    out, lse = pkg.paged_decode(**c, workspace=ws, weights=weights, weight_decay=0.5, return_lse=True)
+    ref = R.decode(c["q"], c["k_pool"], c["v_pool"], c["page_table"], c["kv_lens"], c["rows"], weights=before, decay=0.5)
+    R.within(out, ref["out"], ref["out_tol"])
+    R.within(lse, ref["lse"], ref["lse_tol"])
+    done = c["rows"][:fit].long()
+    R.within(weights[done], ref["weights"][done], ref["weights_tol"][done])
+    before[done] = weights[done]
+    assert torch.equal(weights, before)
+    assert ws.status() == (0 if fit == 3 else -3)
