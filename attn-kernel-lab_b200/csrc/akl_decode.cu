@@ -855,6 +855,7 @@ int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
   if (c->rows == nullptr && c->table_rows < c->batch) return AKL_ERR_INVALID;
   if (c->q_heads % c->kv_heads || c->q_heads / c->kv_heads > kMaxGroup) return AKL_ERR_UNSUPPORTED;
   if (c->pool_rows >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;      // slots travel in 32 bits
+  if (c->table_width >= (1 << 30)) return AKL_ERR_UNSUPPORTED;      // positions too, and loops step past the end
   if (c->kv_heads != 1 && c->kv_heads != 2 && c->kv_heads != 4 && c->kv_heads != 8) return AKL_ERR_UNSUPPORTED;
   if (c->k_stride < c->kv_heads * 256 || c->v_stride < c->kv_heads * 256 || c->q_stride < c->q_heads * 256 ||
       c->table_stride < c->table_width)

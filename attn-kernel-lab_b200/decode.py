@@ -185,6 +185,13 @@ def _check_table(name, t) -> None:
         _reject(f"{name} shape {tuple(t.shape)} exceeds 32 bits", field=name, value=tuple(t.shape), supported="< 2^31")
 
 
+def _check_width(table) -> None:
+    """Positions are 32-bit in the kernels, and loops over them run past the end."""
+    if table.shape[1] >= 1 << 30:
+        _reject(f"page_table rows of {table.shape[1]} entries: at most 2^30 - 1", field="page_table",
+                value=int(table.shape[1]), supported="< 2^30")
+
+
 def _check_batch_vector(name, t, batch, device) -> None:
     _need(name, t, _INDEX, 1, device, "[batch]")
     if t.shape[0] != batch:
@@ -227,6 +234,7 @@ def check_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
     _check_rows("v_pool", v_pool, kv_heads)
     _need("page_table", page_table, _INDEX, 2, device, "[rows, width]")
     _check_table("page_table", page_table)
+    _check_width(page_table)
     _check_batch_vector("kv_lens", kv_lens, batch, device)
     if rows is not None:
         _check_batch_vector("rows", rows, batch, device)
@@ -381,7 +389,7 @@ def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, we
         kv_type, idx_type, lens_type = _KV[k_pool.dtype], _INDEX[page_table.dtype], _INDEX[kv_lens.dtype]
         if (index < 0 or heads != q_heads or kv != kv_heads or dim != 256 or kv_dim != 256
                 or not 1 <= batch <= max_requests or not 1 <= pool < 1 << 31 or not 1 <= table_rows < 1 << 31
-                or not 1 <= width < 1 << 31 or v_pool.shape != pool_shape or v_pool.dtype is not k_pool.dtype
+                or not 1 <= width < 1 << 30 or v_pool.shape != pool_shape or v_pool.dtype is not k_pool.dtype
                 or q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q_shape
                 or kv_lens.shape != (batch,)
                 or not (q.is_contiguous() and k_pool.is_contiguous() and v_pool.is_contiguous()

@@ -18,8 +18,8 @@ import torch
 from . import kernel
 from .capability import DECODE_CAPABILITY, OperatorCapability
 from .decode import (_INDEX, _KV, _Scratch, _call, _check_batch_vector, _check_decay, _check_heads, _check_rows,
-                     _check_scale, _check_sizes, _check_table, _declares, _need, _need_cuda, _overlap, _pool_stride,
-                     _raise_on_status, _row_stride)
+                     _check_scale, _check_sizes, _check_table, _check_width, _declares, _need, _need_cuda, _overlap,
+                     _pool_stride, _raise_on_status, _row_stride)
 from .ops import _dtype_name, _reject, _same_device
 
 __all__ = ["WeightsWorkspace", "evict_lightest", "extend_weights", "plan_weights_workspace"]
@@ -210,9 +210,7 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
     _need("weights", weights, (torch.float32,), 2, device, "[rows, >= width]")
     _check_table("weights", weights)
     width = page_table.shape[1]
-    if width >= 1 << 30:
-        _reject(f"page_table rows of {width} entries: at most 2^30 - 1", field="page_table", value=width,
-                supported="< 2^30")
+    _check_width(page_table)
     if weights.shape[0] != page_table.shape[0] or weights.shape[1] < width:
         _reject(f"weights shape {tuple(weights.shape)} must cover the page table's {tuple(page_table.shape)}",
                 field="weights", value=tuple(weights.shape), supported=tuple(page_table.shape))

@@ -296,7 +296,7 @@ int akl_static_scratch_status(int32_t* host_out, void* stream);
  * with slot(i) = page_table[row][i], row = rows[b] (b itself when rows is NULL).  Lengths, rows and
  * slots are read on the device, so a captured launch follows them.  n is cut to the table's width; a
  * request with n <= 0 or a row outside the table gives out = 0, lse = -inf; a slot outside the pool is
- * skipped.  With weights, no two requests of a call may name the same row. */
+ * skipped.  table_width is below 2^30.  With weights, no two requests of a call may name the same row. */
 typedef struct akl_decode_plan {
   int32_t max_requests;
   int32_t q_heads;
