@@ -93,6 +93,7 @@ constexpr uint64_t kPartBytes = static_cast<uint64_t>(2 * kMaxCtas) * kSlotHeads
 int decode_layout(const akl_decode_plan_t& p, akl_decode_layout_t* o) {
   if (p.max_requests < 1 || p.q_heads < 1 || p.kv_heads < 1 || p.max_weight_tokens < 0) return AKL_ERR_INVALID;
   if (p.q_heads % p.kv_heads || p.q_heads / p.kv_heads > kMaxGroup) return AKL_ERR_UNSUPPORTED;
+  if (p.max_weight_tokens >= (1ll << 40)) return AKL_ERR_UNSUPPORTED;      // beyond any memory, and the bytes stay within 64 bits
   std::memset(o, 0, sizeof(*o));
   uint64_t off = 1024;
   o->off_parts = off;

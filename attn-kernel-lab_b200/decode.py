@@ -58,10 +58,11 @@ class _Scratch:
 
 
 def _check_sizes(**sizes) -> None:
+    """Within the fields that carry them: ctypes would cut a larger number to its low bits without a word."""
     for name, value in sizes.items():
-        low = 0 if name == "max_weight_tokens" else 1
-        if isinstance(value, bool) or not isinstance(value, int) or value < low:
-            raise ValueError(f"{name} must be an int >= {low}, got {value!r}")
+        low, high = (0, 1 << 40) if name == "max_weight_tokens" else (1, 1 << 31)
+        if isinstance(value, bool) or not isinstance(value, int) or not low <= value < high:
+            raise ValueError(f"{name} must be an int >= {low} and below 2^{high.bit_length() - 1}, got {value!r}")
 
 
 class DecodeWorkspace(_Scratch):

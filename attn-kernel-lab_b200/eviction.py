@@ -72,6 +72,9 @@ def _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace,
     if kv_len < 1 or not idx.is_contiguous():
         _reject(f"idx must be contiguous and name at least one position, got {kv_len} with stride {idx.stride()}",
                 field="idx", value=kv_len, supported=">= 1, contiguous")
+    if kv_len >= 1 << 30 or q_len >= 1 << 27:
+        _reject(f"{q_len} rows over {kv_len} positions: at most 2^27 - 1 over 2^30 - 1", field="idx", value=(q_len, kv_len),
+                supported="< 2^27 rows, < 2^30 positions")
     if isinstance(prefix, bool) or not isinstance(prefix, int):
         _reject(f"prefix must be a Python int, got {type(prefix).__name__}", field="prefix",
                 value=type(prefix).__name__, supported="int")
@@ -327,7 +330,7 @@ def _ordinary_evict(page_table, weights, kv_lens, keep, first, last, rows, table
                 or weights.shape != shape or weights.dtype is not torch.float32
                 or type(keep) is not int or type(first) is not int or type(last) is not int
                 or first < 0 or last < 0 or not max(1, first + last) <= keep < 1 << 31
-                or freed_rows != batch or freed_width < max(1, width - keep) or freed.dtype is not page_table.dtype
+                or freed_rows != batch or not max(1, width - keep) <= freed_width < 1 << 31 or freed.dtype is not page_table.dtype
                 or freed_lens.shape != (batch,) or freed_lens.dtype is not torch.int32
                 or not (page_table.is_contiguous() and weights.is_contiguous() and kv_lens.is_contiguous()
                         and freed.is_contiguous() and freed_lens.is_contiguous())

@@ -302,7 +302,7 @@ typedef struct akl_decode_plan {
   int32_t q_heads;
   int32_t kv_heads;
   int32_t reserved_;
-  int64_t max_weight_tokens;  /* sum over a batch of the lengths, each rounded up to 64; 0: no weights */
+  int64_t max_weight_tokens;  /* sum over a batch of the lengths, each rounded up to 64; 0: no weights; below 2^40 */
 } akl_decode_plan_t;
 
 typedef struct akl_decode_layout {

@@ -70,3 +70,30 @@ def test_the_short_form_leaves_wide_tables_alone(pkg, short):      # noqa: F811
                                 None, 1.0, None, False)
 
     assert packed((1 << 30) - 1) is not None and packed(1 << 30) is None and packed((1 << 31) - 1) is None
+
+
+def test_plans_refuse_sizes_that_their_fields_cut(pkg, K):
+    """2^32 + 5 requests would be planned for as 5, and 2^60 tokens take a workspace of nearly nothing."""
+    for over in (dict(max_requests=1 << 31), dict(max_requests=(1 << 32) + 5), dict(max_weight_tokens=1 << 40),
+                 dict(max_weight_tokens=1 << 60), dict(max_weight_tokens=1 << 64), dict(q_heads=(1 << 32) + 24)):
+        with pytest.raises(ValueError):
+            pkg.DecodeWorkspace("meta", **dict(dict(max_requests=1, q_heads=24, kv_heads=4), **over))
+    for over in (dict(max_kv_len=(1 << 32) + 64), dict(max_q_len=(1 << 32) + 1)):
+        with pytest.raises(ValueError):
+            pkg.WeightsWorkspace("meta", **dict(dict(max_kv_len=64, max_q_len=1, q_heads=24, kv_heads=4), **over))
+    lib, L = K.load(), K.DecodeLayout()
+    for tokens, code in (((1 << 40) - 1, 0), (1 << 40, -2), (1 << 60, -2), ((1 << 63) - 1, -2), (-1, -1)):
+        assert lib.akl_decode_layout(ctypes.byref(K.DecodePlan(4, 64, 8, 0, tokens)), ctypes.byref(L)) == code
+        if code == 0:
+            assert L.total_bytes - L.off_scores >= tokens * 64 * 4
+
+
+def test_extends_beyond_32_bit_positions_are_refused(pkg):
+    n = 1 << 30
+    kw = dict(k_pool=torch.empty((4, 4, 256), dtype=torch.bfloat16, device="meta"), prefix=0)
+    for rows, size in ((1, n), (1 << 27, 1 << 28), (1, (1 << 32) + 3)):
+        q = torch.empty((rows, 24, 256), dtype=torch.bfloat16, device="meta")
+        with pytest.raises(pkg.CapabilityError) as e:
+            pkg.extend_weights(q=q, idx=torch.empty(size, dtype=torch.int32, device="meta"),
+                               lse=torch.empty((rows, 24), device="meta"), weights=torch.empty(size, device="meta"), **kw)
+        assert e.value.field == "idx"
