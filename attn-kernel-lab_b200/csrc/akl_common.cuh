@@ -351,6 +351,36 @@ __device__ __forceinline__ long long load_index(const void* idx, int dtype, long
                               : static_cast<long long>(__ldg(reinterpret_cast<const int*>(idx) + i));
 }
 inline bool known_index(int dtype) { return dtype == AKL_IDX_I64 || dtype == AKL_IDX_I32; }
+inline int index_bytes(int dtype) { return dtype == AKL_IDX_I64 ? 8 : 4; }
+
+// Memory of an argument, for the checks on the host: `rows` rows of `bytes` each, `pitch` bytes apart.
+struct Span {
+  const void* at;
+  int64_t rows, bytes, pitch;
+};
+// Whether two of them share a byte, or may: rows side by side in one buffer are told apart, other mixtures of
+// rows are not.  A null pointer shares nothing.
+inline bool meet(const Span& a, const Span& b) {
+  if (a.at == nullptr || b.at == nullptr) return false;
+  using wide = __int128;
+  const wide a0 = reinterpret_cast<uintptr_t>(a.at), b0 = reinterpret_cast<uintptr_t>(b.at);
+  if (a0 + static_cast<wide>(a.rows - 1) * a.pitch + a.bytes <= b0 || b0 + static_cast<wide>(b.rows - 1) * b.pitch + b.bytes <= a0)
+    return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+  const wide pitch = a.rows > 1 ? a.pitch : b.pitch, apart = ((b0 - a0) % pitch + pitch) % pitch;
+  return apart < a.bytes || apart + b.bytes > pitch;
+}
+// Whether one of the outputs meets an input or another output.
+inline bool outputs_meet(const Span* outputs, int n_outputs, const Span* inputs, int n_inputs) {
+  for (int i = 0; i < n_outputs; ++i) {
+    for (int k = 0; k < i; ++k)
+      if (meet(outputs[i], outputs[k])) return true;
+    for (int k = 0; k < n_inputs; ++k)
+      if (meet(outputs[i], inputs[k])) return true;
+  }
+  return false;
+}
 
 // host-side launchers (one translation unit each)
 int launch_kv_tile_stats(const Geom& g, int kv_dtype, int idx_dtype, cudaStream_t s, bool with_q = false);

@@ -871,7 +871,17 @@ int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
                          reinterpret_cast<uintptr_t>(c->v_pool) | reinterpret_cast<uintptr_t>(c->out);
   if ((mask & 15u) || ((c->k_stride | c->v_stride | c->q_stride) & 7) || (reinterpret_cast<uintptr_t>(c->workspace) & 1023u))
     return AKL_ERR_ALIGN;
-  return AKL_OK;
+  const int64_t batch = c->batch, heads = c->q_heads, dense = static_cast<int64_t>(c->kv_heads) * 512;
+  const Span outputs[3] = {{c->out, 1, batch * heads * 512, 1}, {c->lse_out, 1, batch * heads * 4, 1},
+                           {c->weights, c->table_rows, static_cast<int64_t>(c->table_width) * 4, c->weights_stride * 4}};
+  const Span inputs[6] = {{c->q, batch, heads * 512, c->q_stride * 2},
+                          {c->k_pool, c->pool_rows, dense, c->k_stride * 2},
+                          {c->v_pool, c->pool_rows, dense, c->v_stride * 2},
+                          {c->page_table, c->table_rows, static_cast<int64_t>(c->table_width) * index_bytes(c->idx_dtype),
+                           c->table_stride * index_bytes(c->idx_dtype)},
+                          {c->rows, 1, batch * index_bytes(c->rows_dtype), 1},
+                          {c->kv_lens, 1, batch * index_bytes(c->lens_dtype), 1}};
+  return outputs_meet(outputs, 3, inputs, 6) ? AKL_ERR_INVALID : AKL_OK;
 }
 
 template <int KV, int HB>

@@ -415,6 +415,23 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
     return AKL_ERR_INVALID;
   if (c->table_width >= (1 << 30)) return AKL_ERR_UNSUPPORTED;      // positions are 32-bit, and rounds run past the end
   if (c->freed_width < c->table_width - c->keep) return AKL_ERR_CAPACITY;
+  {
+    const int64_t rows = c->table_rows, width = c->table_width, batch = c->batch, item = index_bytes(c->idx_dtype);
+    const int64_t lens_bytes = batch * index_bytes(c->lens_dtype);
+    const Span table = {c->page_table, rows, width * item, c->table_stride * item}, weights = {c->weights, rows, width * 4, c->weights_stride * 4};
+    const Span lens = {c->kv_lens, 1, lens_bytes, 1}, which = {c->rows, 1, batch * index_bytes(c->rows_dtype), 1};
+    const Span outputs[5] = {{c->page_table_out, rows, width * item, c->table_out_stride * item},
+                             {c->weights_out, rows, width * 4, c->weights_out_stride * 4},
+                             {c->kv_lens_out, 1, lens_bytes, 1},
+                             {c->freed, batch, static_cast<int64_t>(c->freed_width) * item, c->freed_stride * item},
+                             {c->freed_lens, 1, batch * 4, 1}};
+    // what is changed in place is read by its own output alone
+    const bool same_table = c->page_table_out == c->page_table && c->table_out_stride == c->table_stride;
+    const bool same_weights = c->weights_out == c->weights && c->weights_out_stride == c->weights_stride;
+    const Span none = {nullptr, 1, 0, 1};
+    const Span inputs[4] = {same_table ? none : table, same_weights ? none : weights, c->kv_lens_out == c->kv_lens ? none : lens, which};
+    if (outputs_meet(outputs, 5, inputs, 4)) return AKL_ERR_INVALID;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int sms = 0;
   const int rc = device_sm_count(&sms);

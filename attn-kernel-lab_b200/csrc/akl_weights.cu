@@ -594,7 +594,13 @@ int check_weights(const akl_weights_t* c, akl_weights_layout_t* L) {
   const uintptr_t mask = reinterpret_cast<uintptr_t>(c->q) | reinterpret_cast<uintptr_t>(c->k_pool);
   if ((mask & 15u) || ((c->k_stride | c->q_stride) & 7) || (reinterpret_cast<uintptr_t>(c->workspace) & 1023u))
     return AKL_ERR_ALIGN;
-  return AKL_OK;
+  const int64_t rows = c->T, heads = c->q_heads, positions = c->N;
+  const Span output = {c->weights, 1, positions * 4, 1};
+  const Span inputs[4] = {{c->q, rows, heads * 512, c->q_stride * 2},
+                          {c->k_pool, c->pool_rows, static_cast<int64_t>(c->kv_heads) * 512, c->k_stride * 2},
+                          {c->idx, 1, positions * index_bytes(c->idx_dtype), 1},
+                          {c->lse, 1, rows * heads * 4, 1}};
+  return outputs_meet(&output, 1, inputs, 4) ? AKL_ERR_INVALID : AKL_OK;
 }
 
 template <int KV>

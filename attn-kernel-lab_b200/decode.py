@@ -157,16 +157,35 @@ def _check_decay(weight_decay) -> None:
 
 
 def _overlap(a, b) -> bool:
-    """Whether the address ranges of two tensors meet."""
-    if a.device.type == "meta" or b.device.type == "meta":
+    """Whether two tensors share memory, or may: rows side by side in one buffer are told apart, other mixtures
+    of rows are not (as the C entries look at it)."""
+    if a.device.type == "meta" or b.device.type == "meta" or not a.numel() or not b.numel():
         return False
 
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    def span(t):                       # address, rows, bytes of one, bytes from row to row
+        item = t.element_size()
+        rows = t.shape[0] if t.dim() > 1 else 1
+        inner = list(zip(t.shape, t.stride()))[t.dim() > 1:]
+        return t.data_ptr(), rows, (sum((n - 1) * s for n, s in inner) + 1) * item, (t.stride(0) if rows > 1 else 0) * item
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    (a0, a_rows, a_bytes, a_pitch), (b0, b_rows, b_bytes, b_pitch) = span(a), span(b)
+    if a0 + (a_rows - 1) * a_pitch + a_bytes <= b0 or b0 + (b_rows - 1) * b_pitch + b_bytes <= a0:
+        return False
+    pitch = a_pitch or b_pitch
+    if not pitch or (a_pitch and b_pitch and a_pitch != b_pitch):
+        return True
+    apart = (b0 - a0) % pitch
+    return apart < a_bytes or apart + b_bytes > pitch
+
+
+def _check_apart(outputs, inputs) -> None:
+    """Every output has memory of its own: lists of (name, tensor or None)."""
+    outputs = [(name, t) for name, t in outputs if t is not None]
+    for i, (name, t) in enumerate(outputs):
+        for other, u in inputs + outputs[:i]:
+            if u is not None and _overlap(t, u):
+                _reject(f"{name} must not overlap {other}", field=name, value=f"overlaps {other}",
+                        supported="memory of its own")
 
 
 def _row_stride(t) -> int:
@@ -268,6 +287,9 @@ def check_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
             _reject(f"weights shape {tuple(weights.shape)} must cover the page table's {tuple(page_table.shape)}",
                     field="weights", value=tuple(weights.shape), supported=tuple(page_table.shape))
         _check_decay(weight_decay)
+    _check_apart([("out", out), ("lse_out", lse_out), ("weights", weights)],
+                 [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("page_table", page_table), ("kv_lens", kv_lens),
+                  ("rows", rows)])
     if workspace is not None:
         if not isinstance(workspace, DecodeWorkspace):
             _reject(f"workspace must be a DecodeWorkspace or None, got {type(workspace).__name__}",
@@ -318,7 +340,7 @@ def paged_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
     table row of each request, default its own index) int32 or int64, read on the device.  A length is
     cut to the table's width; a request of length 0 (or less), or with a row outside the table, gives
     zeros and an LSE of -inf; a slot outside the pool is skipped.  Rows of `q`, pool rows and table rows
-    may be strided.
+    may be strided.  `out`, `lse_out` and `weights` share no memory with each other or with an input.
 
     `weights` [rows, >= width] FP32: position i of each request's row becomes `weight_decay` times itself
     plus the sum over the q heads of what they put on it (the sum over i of that is q_heads); 0
@@ -335,7 +357,14 @@ def paged_decode(q, k_pool, v_pool, page_table, kv_lens, *, rows=None, workspace
         packed = _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, workspace, out, lse_out, weights, weight_decay,
                            sm_scale, return_lse)
         if packed is not None:
-            _call(workspace.device_index, kernel.load().akl_paged_decode, "akl_paged_decode", packed)
+            try:
+                _call(workspace.device_index, kernel.load().akl_paged_decode, "akl_paged_decode", packed)
+            except kernel.NativeError as e:
+                if e.code == kernel.AKL_ERR_INVALID:       # tensors that share memory: say which
+                    check_decode(q, k_pool, v_pool, page_table, kv_lens, rows=rows, workspace=workspace, out=out,
+                                 lse_out=lse_out, weights=weights, weight_decay=weight_decay, sm_scale=sm_scale,
+                                 return_lse=return_lse, capability=capability)
+                raise
             if check_status:
                 _raise_on_status(workspace, "akl_paged_decode")
             return (out, lse_out) if return_lse else out
@@ -376,7 +405,8 @@ def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, we
     """The packed call when every argument has its ordinary form -- contiguous tensors of the expected
     types on one GPU, a plan that admits them -- or None: `check_decode` then looks closer, and either
     accepts or says what is wrong.  A single step is short enough for the checks to show (they were 15
-    of 26 us a call), and these few comparisons are the same ones."""
+    of 26 us a call), and these few comparisons are the same ones; that outputs share no memory with
+    anything else is left to the C entry, which refuses before it launches."""
     try:
         if type(ws) is not DecodeWorkspace or not ws._declared:
             return None

@@ -17,7 +17,7 @@ import torch
 
 from . import kernel
 from .capability import DECODE_CAPABILITY, OperatorCapability
-from .decode import (_INDEX, _KV, _Scratch, _call, _check_batch_vector, _check_decay, _check_heads, _check_rows,
+from .decode import (_INDEX, _KV, _Scratch, _call, _check_apart, _check_batch_vector, _check_decay, _check_heads, _check_rows,
                      _check_scale, _check_sizes, _check_table, _check_width, _declares, _need, _need_cuda, _overlap,
                      _pool_stride, _raise_on_status, _row_stride)
 from .ops import _dtype_name, _reject, _same_device
@@ -89,8 +89,7 @@ def _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace,
     if weights.shape[0] != kv_len or not weights.is_contiguous():
         _reject(f"weights must be contiguous [{kv_len}], got {tuple(weights.shape)} with stride {weights.stride()}",
                 field="weights", value=tuple(weights.shape), supported=(kv_len,))
-    if _overlap(weights, lse):
-        _reject("weights must not overlap lse", field="weights", value="aliases lse", supported="memory of its own")
+    _check_apart([("weights", weights)], [("q", q), ("k_pool", k_pool), ("idx", idx), ("lse", lse)])
     _check_decay(weight_decay)
     if sm_scale is not None:
         _check_scale(sm_scale)
@@ -116,6 +115,7 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
         sum over t, h with i <= prefix + t of 2^(sm_scale log2e <q[t, h], k_i> - lse[t, h]).
 
     A row whose `lse` is infinite adds nothing (it saw no key); a slot outside the pool gets no weight.
+    `weights` shares no memory with an input.
     To judge by a window of w rows pass `q[-w:]`, `lse[-w:]` and `prefix + q_len - w`.  The sum has a
     fixed order: equal inputs give equal bits.
 
@@ -124,7 +124,12 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
     if workspace is not None and capability is DECODE_CAPABILITY:
         packed = _ordinary_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale)
         if packed is not None:
-            _call(workspace.device_index, kernel.load().akl_extend_weights, "akl_extend_weights", packed)
+            try:
+                _call(workspace.device_index, kernel.load().akl_extend_weights, "akl_extend_weights", packed)
+            except kernel.NativeError as e:
+                if e.code == kernel.AKL_ERR_INVALID:       # tensors that share memory: say which
+                    _check_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, workspace, sm_scale, capability)
+                raise
             if check_status:
                 _raise_on_status(workspace, "akl_extend_weights")
             return weights
@@ -253,21 +258,15 @@ def _check_evict(page_table, weights, kv_lens, keep, first, last, rows, table_ou
     if freed_lens is not None:
         _need("freed_lens", freed_lens, (torch.int32,), 1, device, "[batch]")
         _check_batch_vector("freed_lens", freed_lens, batch, device)
-    others = [("page_table", page_table), ("page_table_out", table_out), ("weights", weights),
-              ("weights_out", weights_out), ("kv_lens", kv_lens), ("kv_lens_out", lens_out)]
-    if rows is not None:
-        others.append(("rows", rows))
-        if _overlap(lens_out, rows):
-            _reject("kv_lens_out must not overlap rows", field="kv_lens_out", value="overlaps",
-                    supported="kv_lens or a distinct allocation")
-    for name, t in (("freed", freed), ("freed_lens", freed_lens)):
-        if t is None:
-            continue
-        for other, u in others:
-            if _overlap(t, u):
-                _reject(f"{name} must not overlap {other}", field=name, value="overlaps",
-                        supported="a distinct allocation")
-        others.append((name, t))
+    # an output in place of its input is the one thing they may share (the checks above)
+    for name, t, own in (("page_table_out", table_out, page_table), ("weights_out", weights_out, weights),
+                         ("kv_lens_out", lens_out, kv_lens)):
+        _check_apart([(name, t)], [(other, u) for other, u in (("page_table", page_table), ("weights", weights),
+                                                               ("kv_lens", kv_lens), ("rows", rows)) if u is not own])
+    _check_apart([("page_table_out", table_out), ("weights_out", weights_out), ("kv_lens_out", lens_out), ("freed", freed),
+                  ("freed_lens", freed_lens)], [])
+    _check_apart([("freed", freed), ("freed_lens", freed_lens)],
+                 [("page_table", page_table), ("weights", weights), ("kv_lens", kv_lens), ("rows", rows)])
 
 
 def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: int = 0, protect_last: int = 0, rows=None,
@@ -283,7 +282,8 @@ def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: in
 
     By default `page_table`, `weights` and `kv_lens` are changed in place; `page_table_out`,
     `weights_out` and `kv_lens_out` of the same shapes take the result instead (other rows, and what lies
-    behind a request's old length, stay as they are).  `freed` [batch, >= width - keep] receives the
+    behind a request's old length, stay as they are).  But for that, no output shares memory with an input or
+    another output; a table and its weights may lie side by side in one buffer.  `freed` [batch, >= width - keep] receives the
     slots that go, in position order, and `freed_lens` [batch] int32 their number; both are allocated
     when not given.  Enqueues on the current stream and does not synchronise.
 
@@ -310,7 +310,13 @@ def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: in
             _row_stride(page_table), _row_stride(weights), _row_stride(table_out), _row_stride(acc_out),
             _row_stride(freed), batch, table_rows, width, freed.shape[1], keep, protect_first, protect_last,
             _INDEX[page_table.dtype], 0 if rows is None else _INDEX[rows.dtype], _INDEX[kv_lens.dtype])
-    _call(index, kernel.load().akl_evict_lightest, "akl_evict_lightest", packed)
+    try:
+        _call(index, kernel.load().akl_evict_lightest, "akl_evict_lightest", packed)
+    except kernel.NativeError as e:
+        if e.code == kernel.AKL_ERR_INVALID:               # tensors that share memory: say which
+            _check_evict(page_table, weights, kv_lens, keep, protect_first, protect_last, rows, table_out, acc_out, lens_out,
+                         freed, freed_lens)
+        raise
     return table_out, acc_out, lens_out, freed, freed_lens
 
 

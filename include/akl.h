@@ -10,6 +10,8 @@
  * Conventions (every entry point):
  *   - plain C types, raw device pointers, byte sizes; no tensor-library types;
  *   - returns 0 (AKL_OK) or a negative AKL_ERR_* code, never throws, never traps;
+ *   - decode, weights and eviction: outputs that share memory with an input or with each other are
+ *     AKL_ERR_INVALID, but for an eviction's in place;
  *   - enqueues on the caller's stream and returns; never synchronises
  *     (docs/OPERATOR_CONTRACT.md:210-211 of the reference);
  *   - allocates no device memory: the caller owns inputs, outputs and the workspace

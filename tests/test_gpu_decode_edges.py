@@ -55,3 +55,44 @@ def test_weights_beyond_the_plan_leave_whole_rows_alone(pkg, cuda, tokens, fit):
     before[done] = weights[done]
     assert torch.equal(weights, before)
     assert ws.status() == (0 if fit == 3 else -3)
+
+
+def test_outputs_in_other_memory_are_refused_and_neighbours_are_not(pkg, cuda):
+    """With a workspace and outputs of its own, as an engine calls it."""
+    c = R.case([100, 40], 24, 4, seed=30)
+    ws = pkg.plan_decode_workspace(cuda, max_requests=2, q_heads=24, kv_heads=4, max_weight_tokens=256)
+    out, lse = torch.empty_like(c["q"]), torch.empty((2, 24), device=cuda)
+    weights = torch.zeros(c["page_table"].shape, device=cuda)
+    kw = dict(workspace=ws, lse_out=lse, return_lse=True)
+    for field, over in (("out", dict(out=c["k_pool"].view(-1)[:2 * 24 * 256].view(2, 24, 256))), ("lse_out", dict(out=out, lse_out=out.view(-1).view(torch.float32)[:48].view(2, 24))),
+                        ("weights", dict(out=out, weights=c["page_table"].view(torch.float32)))):
+        with pytest.raises(pkg.CapabilityError) as e:
+            pkg.paged_decode(**c, **dict(kw, **over))
+        assert e.value.field == field
+    # table and weights side by side in one buffer, the outputs one behind the other in another
+    rows, width = c["page_table"].shape
+    both = torch.zeros((rows, 2 * width), dtype=I32, device=cuda)
+    both[:, :width] = c["page_table"]
+    flat = torch.zeros(2 * 24 * 256 + 96, dtype=BF16, device=cuda)
+    got = pkg.paged_decode(**dict(c, page_table=both[:, :width]), workspace=ws, out=flat[:-96].view(2, 24, 256),
+                           lse_out=flat[-96:].view(torch.float32).view(2, 24), return_lse=True, weights=both[:, width:].view(torch.float32))
+    want = pkg.paged_decode(**c, **kw, out=out, weights=weights)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(both[:, width:].view(torch.float32), weights)
+    assert torch.equal(both[:, :width], c["page_table"])
+    lens = c["kv_lens"].clone()
+    pkg.evict_lightest(both[:, :width], both[:, width:].view(torch.float32), lens, keep=30, rows=c["rows"])
+    want = R.evict(c["page_table"].cpu(), weights.cpu(), [100, 40], 30, rows=c["rows"].tolist())
+    assert torch.equal(both[:, :width].cpu(), want[0]) and torch.equal(both[:, width:].view(torch.float32).cpu(), want[1])
+    # eviction and the extend's weights, in their short forms
+    t, n = c["page_table"].clone(), c["kv_lens"].clone()
+    freed, counts = torch.zeros((2, max(1, width - 30)), dtype=I32, device=cuda), torch.zeros(2, dtype=I32, device=cuda)
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.evict_lightest(t, weights, n, keep=30, rows=c["rows"], freed=freed, freed_lens=counts, page_table_out=torch.zeros_like(t),
+                           weights_out=t.view(torch.float32))
+    assert e.value.field == "weights_out"
+    q = c["q"][:2].contiguous()
+    idx = c["page_table"][c["rows"][0].long(), :100].contiguous()
+    wws = pkg.plan_weights_workspace(cuda, max_kv_len=128, max_q_len=2, q_heads=24, kv_heads=4)
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.extend_weights(q, c["k_pool"], idx, 98, lse, idx.view(torch.float32), workspace=wws)
+    assert e.value.field == "weights"
