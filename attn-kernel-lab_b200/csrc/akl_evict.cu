@@ -20,8 +20,8 @@
 // position, at 60 % of the issue slots.
 #include <cooperative_groups.h>
 
-#include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "akl_common.cuh"
 
@@ -34,7 +34,6 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kStep = 8, kGroups = 4;           // positions of a thread: groups of up to eight steps
 constexpr int kCap = kThreads * kStep * kGroups;
-constexpr int kMaxCluster = 16;
 constexpr int kBins = 2048;
 constexpr int kSorted = kThreads;              // requests that are put in order of their lengths, at most
 
@@ -369,28 +368,78 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
   }
 }
 
-template <typename Slot>
-int launch_evict(const akl_evict_t& c, int ctas, bool longest_first, cudaStream_t s) {
-  static std::atomic<bool> configured[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && !(dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire))) {
-    e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCap * 4);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
-  }
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+// Clusters of 2, 4, 8 and 16 CTAs that the current device holds at once (a cluster lies within one of its
+// groups of SMs, so that is less than their number over the cluster's); 0 where it takes none of that size.
+struct Held {
+  int clusters[4];
+};
+
+cudaLaunchConfig_t launch_config(int requests, int ctas, cudaStream_t s, cudaLaunchAttribute* attr) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(c.batch) * ctas);
+  cfg.gridDim = dim3(static_cast<unsigned>(requests) * ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kCap * 4;
   cfg.stream = s;
-  cfg.attrs = &attr;
+  cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, evict_kernel<Slot>, c, longest_first);
+  return cfg;
+}
+
+// Once a device: the kernel's attributes, and what the device holds of it.
+template <typename Slot>
+cudaError_t configure(Held* out) {
+  static std::atomic<bool> configured[64];
+  static Held held[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && configured[dev].load(std::memory_order_acquire)) { *out = held[dev]; return e; }
+  e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_kernel<Slot>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCap * 4);
+  if (e != cudaSuccess) return e;
+  for (int i = 0; i < 4; ++i) {
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = launch_config(1, 2 << i, nullptr, &attr);
+    out->clusters[i] = 0;
+    if (cudaOccupancyMaxActiveClusters(&out->clusters[i], evict_kernel<Slot>, &cfg) != cudaSuccess) {
+      out->clusters[i] = 0;
+      cudaGetLastError();                               // a size that the device does not take is no error of this call
+    }
+  }
+  if (known) {
+    static std::mutex mutex;
+    std::lock_guard<std::mutex> lock(mutex);
+    held[dev] = *out;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  return e;
+}
+
+template <typename Slot>
+int launch_evict(const akl_evict_t& c, int sms, cudaStream_t s) {
+  Held held;
+  cudaError_t e = configure<Slot>(&held);
+  if (e != cudaSuccess) { note_cuda_error(e, "evict_kernel"); return AKL_ERR_CUDA; }
+  // Clusters while the device holds one for every request at once, but at least two steps for every thread of the widest row.
+  // (256 requests of up to 32768: 55 us with a CTA each, 71 with two, 108 with four; one of 139264: 177, 102, 58,
+  // 30 and 24 us with 1, 2, 4, 8 and 16.  Counted by SMs alone, 8 or 9 requests of 40000 got clusters of 16 of which
+  // one had to wait for another to end: 27.6 us, and 13.9 now; 16 requests 25.7 and 17.6, 36 requests 31.9 and 22.7.)
+  int ctas = 1;
+  for (int i = 0; i < 4 && c.batch <= held.clusters[i] && c.table_width > 2 * kThreads * ctas; ++i) ctas *= 2;
+  if (static_cast<int64_t>(c.batch) * ctas >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
+  // More requests than SMs: the long ones first, or the last to start could be the longest (47 us became 41, and 38 with
+  // the comparisons that order them shared out among the threads).
+  // Every CTA then reads all lengths, so not where the first ones to finish overwrite them.
+  const int64_t lens_bytes = static_cast<int64_t>(c.batch) * (c.lens_dtype == AKL_IDX_I64 ? 8 : 4);
+  const int64_t apart = static_cast<const char*>(c.kv_lens_out) - static_cast<const char*>(c.kv_lens);
+  const bool longest_first = ctas == 1 && c.batch > sms && c.batch <= kSorted && c.table_width < (1 << 21) && (apart >= lens_bytes || -apart >= lens_bytes);
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg = launch_config(c.batch, ctas, s, &attr);
+  e = cudaLaunchKernelEx(&cfg, evict_kernel<Slot>, c, longest_first);
   if (e != cudaSuccess) { note_cuda_error(e, "evict_kernel"); return AKL_ERR_CUDA; }
   return AKL_OK;
 }
@@ -436,18 +485,5 @@ extern "C" int akl_evict_lightest(const akl_evict_t* c, void* stream) {
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != AKL_OK) return rc;
-  // Clusters while the requests leave SMs idle, but at least two steps for every thread of the widest row.
-  // (256 requests of up to 32768: 55 us with a CTA each, 71 with two, 108 with four; one of 139264: 177, 102, 58,
-  // 30 and 24 us with 1, 2, 4, 8 and 16.)
-  int ctas = 1;
-  while (ctas < kMaxCluster && static_cast<int64_t>(c->batch) * ctas * 2 <= sms && c->table_width > 2 * kThreads * ctas) ctas *= 2;
-  if (static_cast<int64_t>(c->batch) * ctas >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
-  // More requests than SMs: the long ones first, or the last to start could be the longest (47 us became 41, and 38 with
-  // the comparisons that order them shared out among the threads).
-  // Every CTA then reads all lengths, so not where the first ones to finish overwrite them.
-  const int64_t lens_bytes = static_cast<int64_t>(c->batch) * (c->lens_dtype == AKL_IDX_I64 ? 8 : 4);
-  const int64_t apart = static_cast<const char*>(c->kv_lens_out) - static_cast<const char*>(c->kv_lens);
-  const bool longest_first = ctas == 1 && c->batch > sms && c->batch <= kSorted && c->table_width < (1 << 21) && (apart >= lens_bytes || -apart >= lens_bytes);
-  return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, ctas, longest_first, s)
-                                     : launch_evict<int>(*c, ctas, longest_first, s);
+  return c->idx_dtype == AKL_IDX_I64 ? launch_evict<long long>(*c, sms, s) : launch_evict<int>(*c, sms, s);
 }

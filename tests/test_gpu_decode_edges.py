@@ -96,3 +96,23 @@ def test_outputs_in_other_memory_are_refused_and_neighbours_are_not(pkg, cuda):
     with pytest.raises(pkg.CapabilityError) as e:
         pkg.extend_weights(q, c["k_pool"], idx, 98, lse, idx.view(torch.float32), workspace=wws)
     assert e.value.field == "weights"
+
+
+@pytest.mark.parametrize("batch", [8, 9, 10, 17, 18, 19, 37, 74, 75, 149])
+def test_eviction_whatever_clusters_the_device_holds_at_once(pkg, cuda, batch):
+    """Requests just below and above what fits the GPU in clusters of sixteen, eight, four, two and one."""
+    width, keep = 33000, 900
+    g = torch.Generator().manual_seed(batch)
+    table = torch.randint(0, 1 << 30, (batch, width), generator=g).to(I32)
+    w = torch.exp(2 * torch.randn((batch, width), generator=g))
+    lens = [width - 17 * i for i in range(batch)]
+    t, a, n = table.to(cuda), w.to(cuda), torch.tensor(lens, dtype=I32, device=cuda)
+    _, _, _, freed, counts = pkg.evict_lightest(t, a, n, keep=keep, protect_first=2, protect_last=30)
+    for b, length in enumerate(lens):
+        middle = torch.arange(2, length - 30)
+        order = middle[torch.sort(w[b, 2:length - 30], descending=True, stable=True).indices[:keep - 32]]
+        stays = torch.zeros(length, dtype=torch.bool)
+        stays[:2] = stays[length - 30:] = stays[order] = True
+        assert torch.equal(t[b, :keep].cpu(), table[b, :length][stays]) and torch.equal(a[b, :keep].cpu(), w[b, :length][stays])
+        assert torch.equal(freed[b, :length - keep].cpu(), table[b, :length][~stays]) and not a[b, keep:length].any()
+    assert n.tolist() == [keep] * batch and counts.tolist() == [x - keep for x in lens]
