@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const akl_weights_t c, u
     for (int i = 0; i < 8; ++i) {
       const int row = row0 + half + i;
       float factor = c.sm_scale * (kLog2e * kGiveBack);
+      if (isinf(lse[i])) raw[i] = make_uint4(0u, 0u, 0u, 0u);     // saw no key, or is no row: whatever it holds, its scores are 0
       uint4 out = raw[i];
       if (KV == AKL_KV_FP16) {
         float x[8], top = 0.f;
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const akl_weights_t c, u
       if (lane == 0) {
         float* f = reinterpret_cast<float*>(image + kImage);
         f[row] = factor;
-        f[kRows + row] = isinf(lse[i]) ? -INFINITY : -lse[i];      // a row that saw no key, or is none, adds nothing
+        f[kRows + row] = isinf(lse[i]) ? -INFINITY : -lse[i];      // and add nothing
       }
     }
     for (int i = 0; i < 8; ++i)

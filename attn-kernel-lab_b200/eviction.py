@@ -114,7 +114,8 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
 
         sum over t, h with i <= prefix + t of 2^(sm_scale log2e <q[t, h], k_i> - lse[t, h]).
 
-    A row whose `lse` is infinite adds nothing (it saw no key); a slot outside the pool gets no weight.
+    A row whose `lse` is infinite adds nothing, whatever its `q` holds (it saw no key); a key that is not finite
+    makes its own position's weight NaN as soon as a row sees it, and no other's; a slot outside the pool gets no weight.
     `weights` shares no memory with an input.
     To judge by a window of w rows pass `q[-w:]`, `lse[-w:]` and `prefix + q_len - w`.  The sum has a
     fixed order: equal inputs give equal bits.

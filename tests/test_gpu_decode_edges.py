@@ -116,3 +116,22 @@ def test_eviction_whatever_clusters_the_device_holds_at_once(pkg, cuda, batch):
         assert torch.equal(t[b, :keep].cpu(), table[b, :length][stays]) and torch.equal(a[b, :keep].cpu(), w[b, :length][stays])
         assert torch.equal(freed[b, :length - keep].cpu(), table[b, :length][~stays]) and not a[b, keep:length].any()
     assert n.tolist() == [keep] * batch and counts.tolist() == [x - keep for x in lens]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("blind", [math.inf, -math.inf])
+def test_rows_without_a_finite_lse_add_nothing_whatever_they_hold(pkg, cuda, dtype, blind):
+    from test_gpu_decode import extend_case
+
+    c = extend_case(70, 200, 24, 4, dtype=dtype, seed=25)
+    for row, head, value in ((3, 5, math.nan), (40, 0, math.inf), (41, 23, -math.inf), (69, 7, 3e38)):
+        c["q"][row, head], c["lse"][row, head] = value, blind
+    c["q"][12, 8, 17], c["lse"][12, 8] = math.nan, blind
+    kept = c["q"].nan_to_num(0.0, 0.0, 0.0)
+    want, tol = R.extend_weights(kept, c["k_pool"], c["idx"], 200, c["lse"], torch.zeros(270, device=cuda), 0.0)
+    got = pkg.extend_weights(**c, weights=torch.zeros(270, device=cuda), weight_decay=0.0)
+    R.within(got, want, tol)
+    c["k_pool"][c["idx"][100].long(), 1, 3] = math.inf          # one position's key: seen by every row
+    got = pkg.extend_weights(**c, weights=torch.zeros(270, device=cuda), weight_decay=0.0)
+    others = torch.arange(270, device=cuda) != 100
+    R.within(got[others], want[others], tol[others])
