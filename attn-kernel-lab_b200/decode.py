@@ -12,7 +12,6 @@ are those of `ops.prefill_extend`.  Nothing here loads the native library before
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -24,6 +23,7 @@ __all__ = ["DecodeWorkspace", "check_decode", "paged_decode", "plan_decode_works
 
 _INDEX = {torch.int64: 0, torch.int32: 1}          # AKL_IDX_*
 _KV = {torch.bfloat16: 0, torch.float16: 1}        # AKL_KV_*
+_SCALES = 2.0 ** -126, 2.0 ** 127                  # sm_scale and sm_scale log2e are normal 32-bit numbers
 _CHUNK = 64                                        # positions per chunk of recorded scores
 
 
@@ -145,9 +145,9 @@ def _check_scale(sm_scale) -> None:
     if isinstance(sm_scale, bool) or not isinstance(sm_scale, (int, float)):
         _reject(f"sm_scale must be a real number or None, got {type(sm_scale).__name__}", field="sm_scale",
                 value=type(sm_scale).__name__, supported="float | None")
-    if not math.isfinite(sm_scale) or sm_scale <= 0.0:
-        _reject(f"sm_scale must be positive and finite, got {sm_scale!r}", field="sm_scale", value=sm_scale,
-                supported="> 0, finite")
+    if not _SCALES[0] <= sm_scale <= _SCALES[1]:
+        _reject(f"sm_scale must be positive, finite and within 32 bits, got {sm_scale!r}", field="sm_scale", value=sm_scale,
+                supported=_SCALES)
 
 
 def _check_decay(weight_decay) -> None:
@@ -453,7 +453,7 @@ def _ordinary(q, k_pool, v_pool, page_table, kv_lens, rows, ws, out, lse_out, we
             weights_ptr = weights.data_ptr()
         if sm_scale is None:
             sm_scale = 0.0625
-        elif type(sm_scale) is not float or not 0.0 < sm_scale < math.inf:
+        elif type(sm_scale) is not float or not 2.0 ** -126 <= sm_scale <= 2.0 ** 127:
             return None
         q_ptr, k_ptr, v_ptr, out_ptr = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
         row = heads * 256

@@ -11,7 +11,6 @@ The reference has no counterpart; validation, errors, workspaces and streams are
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -180,7 +179,7 @@ def _ordinary_extend(q, k_pool, idx, prefix, lse, weights, weight_decay, ws, sm_
                 or not 1 <= kv_len <= max_kv_len or pool < 1 or type(prefix) is not int or not 0 <= prefix <= kv_len - q_len
                 or q.dtype is not torch.bfloat16 or lse.dtype is not torch.float32 or lse.shape != (q_len, heads)
                 or weights.dtype is not torch.float32 or weights.shape != (kv_len,)
-                or type(sm_scale) is not float or not 0.0 < sm_scale < math.inf
+                or type(sm_scale) is not float or not 2.0 ** -126 <= sm_scale <= 2.0 ** 127
                 or type(weight_decay) is not float or not 0.0 <= weight_decay <= 1.0
                 or not (q.is_contiguous() and k_pool.is_contiguous() and idx.is_contiguous() and lse.is_contiguous()
                         and weights.is_contiguous())

@@ -243,3 +243,24 @@ def test_c_entries_refuse_shared_memory(K):
         if (first, second) == ("kv_lens", "kv_lens_out"):
             call.kv_lens_out = call.kv_lens + 8            # at its first byte it would be in place
         assert lib.akl_evict_lightest(ctypes.byref(call), None) == -1, (first, second)
+
+
+@pytest.mark.parametrize("sm_scale,fits", [(2.0 ** -126, True), (2.0 ** 127, True), (1, True), (2.0 ** -127, False), (1e300, False),
+                                           (1e-300, False), (10 ** 400, False), (float("inf"), False)])
+def test_scales_are_refused_where_32_bits_do_not_hold_them(pkg, short, monkeypatch, sm_scale, fits):      # noqa: F811
+    decode, eviction, seen = short
+    c = decode_ref.case([5, 9], 24, 4, device="cpu")
+    ws = pkg.plan_decode_workspace("cpu", max_requests=2, q_heads=24, kv_heads=4)
+    wws = pkg.plan_weights_workspace("cpu", max_kv_len=20, max_q_len=4, q_heads=24, kv_heads=4)
+    ws.device_index = wws.device_index = 0
+    extend = dict(q=torch.zeros(4, 24, 256, dtype=torch.bfloat16), k_pool=torch.zeros(40, 4, 256, dtype=torch.float16),
+                  idx=torch.arange(20), prefix=16, lse=torch.zeros(4, 24), weights=torch.zeros(20), workspace=wws)
+    for call in (lambda: pkg.paged_decode(**c, workspace=ws, out=torch.zeros(2, 24, 256, dtype=torch.bfloat16), sm_scale=sm_scale),
+                 lambda: pkg.extend_weights(**extend, sm_scale=sm_scale)):
+        if fits:
+            call()
+        else:
+            with pytest.raises(pkg.CapabilityError) as e:
+                call()
+            assert e.value.field == "sm_scale"
+    assert len(seen) == (2 if fits else 0)
