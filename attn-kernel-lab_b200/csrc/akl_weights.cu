@@ -94,7 +94,11 @@ struct Units {
   }
   __host__ __device__ long long start(int p) const {
     long long u = static_cast<long long>(p < full ? p : full) * (tiles + piece);
-    for (int i = full; i < p; ++i) u += cost(i);
+    for (int i = full; i < p; ++i) {
+      const int n = cost(i);
+      if (n == 0) break;                            // seen by no row, as are all behind it
+      u += n;
+    }
     return u * heads;
   }
   // Where cost `at` (below total) falls, and how many units lie before it.

@@ -135,3 +135,29 @@ def test_rows_without_a_finite_lse_add_nothing_whatever_they_hold(pkg, cuda, dty
     got = pkg.extend_weights(**c, weights=torch.zeros(270, device=cuda), weight_decay=0.0)
     others = torch.arange(270, device=cuda) != 100
     R.within(got[others], want[others], tol[others])
+
+
+def test_extend_weights_with_millions_of_positions_that_no_row_sees(pkg, cuda):
+    """They lie behind the last row's diagonal: their weights decay, and no more.  (A call takes 0.12 ms; with a
+    walk over all tiles of positions before each of them it took 33, and minutes at the largest lengths.)"""
+    n, rows, prefix = 1 << 23, 3, 300
+    k = torch.randn((512, 4, 256), device=cuda).to(BF16)
+    q = torch.randn((rows, 24, 256), device=cuda).to(BF16)
+    idx = torch.randint(0, 512, (n,), device=cuda)
+    seen = prefix + rows
+    x = torch.einsum("tjgd,njd->tjgn", q.view(rows, 4, 6, 256).double(), k[idx[:seen]].double()).reshape(rows, 24, seen) / 16
+    hidden = torch.arange(seen, device=cuda) > prefix + torch.arange(rows, device=cuda)[:, None, None]
+    lse = (torch.logsumexp(x.masked_fill(hidden, -math.inf), -1) * R.LOG2E).float()
+    before = torch.rand(n, device=cuda)
+    ws = pkg.plan_weights_workspace(cuda, max_kv_len=n, max_q_len=rows, q_heads=24, kv_heads=4)
+    weights = before.clone()
+    pkg.extend_weights(q, k, idx, prefix, lse, weights, weight_decay=0.5, workspace=ws, check_status=True)
+    want, tol = R.extend_weights(q, k, idx[:seen], prefix, lse, before[:seen], 0.5)
+    R.within(weights[:seen], want, tol)
+    assert torch.equal(weights[seen:], before[seen:] * 0.5)
+    start, stop = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    pkg.extend_weights(q, k, idx, prefix, lse, weights, workspace=ws)
+    stop.record()
+    stop.synchronize()
+    assert start.elapsed_time(stop) < 5.0
