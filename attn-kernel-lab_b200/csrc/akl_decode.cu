@@ -106,6 +106,9 @@ int decode_layout(const akl_decode_plan_t& p, akl_decode_layout_t* o) {
   return AKL_OK;
 }
 
+// CTAs that add a request's weights, 256 positions at a time.
+inline int weight_blocks(const akl_decode_t& c) { return c.weights != nullptr ? std::min((c.table_width + 255) / 256, 64) : 0; }
+
 // What the kernels get besides the call.
 struct Work {
   int* status;
@@ -871,6 +874,9 @@ int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
                          reinterpret_cast<uintptr_t>(c->v_pool) | reinterpret_cast<uintptr_t>(c->out);
   if ((mask & 15u) || ((c->k_stride | c->v_stride | c->q_stride) & 7) || (reinterpret_cast<uintptr_t>(c->workspace) & 1023u))
     return AKL_ERR_ALIGN;
+  // the second launch's CTAs, counted before the first one runs (a wide join has few requests)
+  if ((static_cast<int64_t>(c->batch) * c->q_heads + 7) / 8 + static_cast<int64_t>(c->batch) * weight_blocks(*c) >= (1ll << 31))
+    return AKL_ERR_UNSUPPORTED;
   const int64_t batch = c->batch, heads = c->q_heads, dense = static_cast<int64_t>(c->kv_heads) * 512;
   const Span outputs[3] = {{c->out, 1, batch * heads * 512, 1}, {c->lse_out, 1, batch * heads * 4, 1},
                            {c->weights, c->table_rows, static_cast<int64_t>(c->table_width) * 4, c->weights_stride * 4}};
@@ -958,9 +964,8 @@ int akl_paged_decode(const akl_decode_t* c, void* stream) {
   const int64_t pairs = static_cast<int64_t>(c->batch) * c->q_heads;
   const bool wide = pairs * 4 <= 8 * sms;
   const int64_t joins = wide ? pairs * 4 : (pairs + 7) / 8;
-  const int blocks = c->weights != nullptr ? std::min((c->table_width + 255) / 256, 64) : 0;
+  const int blocks = weight_blocks(*c);
   const int64_t grid = joins + static_cast<int64_t>(c->batch) * blocks;
-  if (grid >= (1ll << 31)) return AKL_ERR_UNSUPPORTED;
   const int hb_heads = hb * (c->q_heads / c->kv_heads);
   return launch_after(wide ? decode_finish_kernel<true> : decode_finish_kernel<false>, dim3(static_cast<unsigned>(grid)), s,
                       "decode_finish_kernel", *c, w, hb_heads, static_cast<int>(joins), blocks);

@@ -264,3 +264,15 @@ def test_scales_are_refused_where_32_bits_do_not_hold_them(pkg, short, monkeypat
                 call()
             assert e.value.field == "sm_scale"
     assert len(seen) == (2 if fits else 0)
+
+
+def test_a_call_whose_second_launch_does_not_fit_is_refused_before_the_first(K):
+    batch = 1 << 26
+    c = _c_decode(K, batch=batch, rows=1, weights=1, table_width=1 << 14, table_stride=1 << 14, weights_stride=1 << 14)
+    c.plan = K.DecodePlan(batch, 24, 4, 0, 64)
+    L = K.DecodeLayout()
+    K.check(K.load().akl_decode_layout(ctypes.byref(c.plan), ctypes.byref(L)), "layout")
+    c.workspace_bytes = int(L.total_bytes)
+    for i, name in enumerate(n for n, t in c._fields_ if t is ctypes.c_void_p):
+        setattr(c, name, (i + 2) << 48)
+    assert K.load().akl_paged_decode(ctypes.byref(c), None) == -2
