@@ -161,3 +161,60 @@ def test_extend_weights_with_millions_of_positions_that_no_row_sees(pkg, cuda):
     stop.record()
     stop.synchronize()
     assert start.elapsed_time(stop) < 5.0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads", [(24, 4), (6, 1), (10, 2)])
+@pytest.mark.parametrize("where", ["some", "tiles", "part", "all"])
+def test_scores_of_minus_infinity_weigh_nothing(pkg, cuda, dtype, heads, where):
+    """Keys of -inf under positive queries, at scattered positions, over whole tiles, over more than a CTA's part of a
+    request, at every position: as if their slots were not there."""
+    c = R.case([700, 5000, 40], *heads, dtype=dtype, seed=33)
+    c["q"] = c["q"].abs().clamp(min=0.01)
+    r = c["rows"].long()
+    gone = torch.zeros(c["page_table"].shape, dtype=torch.bool, device=cuda)
+    if where == "some":
+        gone[r] = torch.rand((3, gone.shape[1]), generator=torch.Generator().manual_seed(4)).to(cuda) < 0.2
+    elif where == "tiles":
+        gone[r[0], 64:192] = gone[r[1], 4992:] = gone[r[2], :16] = True
+    elif where == "part":
+        gone[r[1], :2500] = gone[r[0], 300:] = True
+    else:
+        gone[r[0]] = gone[r[2]] = True
+    for b, n in enumerate((700, 5000, 40)):
+        c["k_pool"][c["page_table"][r[b], :n][gone[r[b], :n]].long()] = -math.inf
+    before = torch.rand(c["page_table"].shape, generator=torch.Generator().manual_seed(5)).to(cuda)
+    weights = before.clone()
+    out, lse = pkg.paged_decode(**c, weights=weights, weight_decay=0.5, return_lse=True, check_status=True)
+    ref = R.decode(c["q"], c["k_pool"], c["v_pool"], torch.where(gone, -1, c["page_table"]), c["kv_lens"], c["rows"], weights=before,
+                   decay=0.5)
+    R.within(out, ref["out"], ref["out_tol"])
+    R.within(lse, ref["lse"], ref["lse_tol"])
+    R.within(weights, ref["weights"], ref["weights_tol"])
+    if where == "all":
+        assert not out[0].any() and bool((lse[2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_weights_of_rows_whose_products_are_exact(pkg, cuda, dtype):
+    """Queries of a few channels: nothing is cut off their scores, of up to some thousands, and little may be added."""
+    g = torch.Generator().manual_seed(6)
+    rows, prefix, n = 40, 260, 300
+    q = torch.zeros((rows, 24, 256))
+    for at in (0, 77, 200):
+        q[:, :, at] = torch.randint(-64, 65, (rows, 24), generator=g) * 4.0
+    k = torch.randint(-16, 17, (n, 4, 256), generator=g).float() * 8
+    q, k = q.to(BF16).to(cuda), k.to(dtype).to(cuda)
+    x = torch.einsum("tjgd,njd->tjgn", q.view(rows, 4, 6, 256).double(), k.double()).reshape(rows, 24, n) / 16
+    hidden = torch.arange(n, device=cuda) > prefix + torch.arange(rows, device=cuda)[:, None, None]
+    x = x.masked_fill(hidden, -math.inf)
+    assert float(x.amax(-1).median()) > 1000
+    lse = (torch.logsumexp(x, -1) * R.LOG2E).float()
+    got = pkg.extend_weights(q, k, torch.arange(n, device=cuda), prefix, lse, torch.zeros(n, device=cuda), weight_decay=0.0)
+    want, tol = R.extend_weights(q, k, torch.arange(n, device=cuda), prefix, lse, torch.zeros(n, device=cuda), 0.0)
+    # (an exponential below 2^-126 may come out as 0: 32 bits hold no normal number there)
+    R.within(got, want, tol + rows * 24 * 2.0 ** -126)
+    # per row and head: half a step of the score and of the LSE, and the 2^-22 that the factor adds on average to make up for
+    # what longer products lose; three roundings of the factor and the exponent's argument besides
+    size = float(x.amax()) * R.LOG2E
+    assert float(((got.double() - want).abs() / want.clamp(min=1e-3)).max()) <= math.log(2) * size * (2.0 ** -22 + 5 * 2.0 ** -24) + 1e-5
