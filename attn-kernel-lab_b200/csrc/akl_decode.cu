@@ -728,18 +728,77 @@ __device__ __forceinline__ void join_wide(const akl_decode_t& c, const Work& w, 
   }
 }
 
-// Many requests, so few parts of each: a warp per (request, q head), a lane eight channels, one part
-// after the other with a running maximum.
-__device__ __forceinline__ void join_warp(const akl_decode_t& c, const Work& w, int hb_heads, int block) {
+// All 256 channels of one (request, q head) by a CTA: four sets of 64 threads take every fourth part, a few of them
+// in flight.  (Registers count here: the weights of a batch are added by this kernel too, and its whole call takes
+// 3 % longer at 80 registers than at 40.)
+__device__ __forceinline__ void join_block(const akl_decode_t& c, const Work& w, long long at, int h, const int4 info) {
+  constexpr int kSets = 4, kFlight = 4;
+  __shared__ float sm_f[kMaxCtas];
+  __shared__ float sm_red[16];
+  __shared__ __align__(16) float sm_o[kSets][256];      // read and written as float4
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int parts = info.z - info.y + 1;
+  auto slot = [&](int i) { return (i == 0 ? info.x : 2 * (info.y + i)) * kSlotHeads + h; };
+  float2 mine = make_float2(-INFINITY, 0.f);
+  if (tid < parts) mine = w.ml[slot(tid)];
+  float top = warp_max(mine.x);
+  if (lane == 0) sm_red[warp] = top;
+  __syncthreads();
+  top = warp_max(sm_red[lane & 7]);
+  const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
+  if (tid < parts) sm_f[tid] = f;
+  float sum = mine.y * f;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  if (lane == 0) sm_red[8 + warp] = sum;
+  __syncthreads();
+  const int set = tid >> 6, ch = (tid & 63) * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = set; i < parts; i += kSets * kFlight) {
+    float4 v[kFlight];
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k)
+      if (i + k * kSets < parts) v[k] = *reinterpret_cast<const float4*>(w.parts + static_cast<long long>(slot(i + k * kSets)) * 256 + ch);
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k)
+      if (i + k * kSets < parts) {
+        const float fi = sm_f[i + k * kSets];
+        o.x = fmaf(fi, v[k].x, o.x);
+        o.y = fmaf(fi, v[k].y, o.y);
+        o.z = fmaf(fi, v[k].z, o.z);
+        o.w = fmaf(fi, v[k].w, o.w);
+      }
+  }
+  *reinterpret_cast<float4*>(&sm_o[set][ch]) = o;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += sm_red[8 + i];
+  const float total = (sm_o[0][tid] + sm_o[1][tid]) + (sm_o[2][tid] + sm_o[3][tid]);
+  reinterpret_cast<__nv_bfloat16*>(c.out)[at * 256 + tid] = __float2bfloat16_rn(sum == 0.f ? 0.f : total / sum);
+  if (tid == 0) {
+    const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    w.lse[at] = lse;
+    if (c.lse_out != nullptr) c.lse_out[at] = lse;
+  }
+  __syncthreads();                                      // the shared memory is the next one's
+}
+
+// Many requests: a warp per (request, q head), a lane eight channels, one part after the other with a running
+// maximum.  That is half a microsecond a part, and a long request among short ones still has a part in nearly every
+// CTA; so a pair of more than kSerial parts is left to the whole CTA (true).  (24:4, one request of 131072 among twelve of 3:
+// 182 us when the warp walked through all its parts, 114 now, and 109 with the wide join of one request fewer; of 8192:
+// 81, 25 and 17 us.)
+constexpr int kSerial = 8;
+__device__ __forceinline__ bool join_warp(const akl_decode_t& c, const Work& w, int hb_heads, long long at) {
   const int lane = threadIdx.x & 31;
-  const long long at = static_cast<long long>(block) * 8 + (threadIdx.x >> 5);
   const bool in = at < static_cast<long long>(c.batch) * c.q_heads;
   const int b = in ? static_cast<int>(at / c.q_heads) : 0, head = in ? static_cast<int>(at - static_cast<long long>(b) * c.q_heads) : 0;
   const int hb = head / hb_heads, h = head - hb * hb_heads;
   long long row;
   const int n = request_of(c, b, row);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!in) return;
+  if (!in) return false;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(c.out) + at * 256 + lane * 8;
   float m = -INFINITY, l = 0.f, o[8];
 #pragma unroll
@@ -747,7 +806,8 @@ __device__ __forceinline__ void join_warp(const akl_decode_t& c, const Work& w, 
   if (n > 0) {
     const int4 info = w.info[b * 2 + hb];
     const int parts = info.z - info.y + 1;
-    if (parts == 1) return;
+    if (parts == 1) return false;
+    if (parts > kSerial) return true;
 #pragma unroll 2
     for (int i = 0; i < parts; ++i) {
       const int s = (i == 0 ? info.x : 2 * (info.y + i)) * kSlotHeads + h;
@@ -775,6 +835,23 @@ __device__ __forceinline__ void join_warp(const akl_decode_t& c, const Work& w, 
     const float lse = l == 0.f ? -INFINITY : m + log2f(l);
     w.lse[at] = lse;
     if (c.lse_out != nullptr) c.lse_out[at] = lse;
+  }
+  return false;
+}
+
+// The pairs of a CTA lie `joins` apart, so that the q heads of one long request fall to different CTAs.
+__device__ __forceinline__ void join_many(const akl_decode_t& c, const Work& w, int hb_heads, int block, int joins) {
+  __shared__ bool sm_long[8];
+  const int warp = threadIdx.x >> 5;
+  const bool left = join_warp(c, w, hb_heads, block + static_cast<long long>(warp) * joins);
+  if ((threadIdx.x & 31) == 0) sm_long[warp] = left;
+  __syncthreads();
+  for (int i = 0; i < 8; ++i) {
+    if (!sm_long[i]) continue;
+    const long long at = block + static_cast<long long>(i) * joins;
+    const int b = static_cast<int>(at / c.q_heads), head = static_cast<int>(at - static_cast<long long>(b) * c.q_heads);
+    const int hb = head / hb_heads, h = head - hb * hb_heads;
+    join_block(c, w, at, h, w.info[b * 2 + hb]);
   }
 }
 
@@ -844,7 +921,7 @@ __global__ void __launch_bounds__(256) decode_finish_kernel(const akl_decode_t c
   const int block = blockIdx.x;
   if (block >= joins) add_weights(c, w, hb_heads, block - joins, blocks);
   else if (kWide) join_wide(c, w, hb_heads, block);
-  else join_warp(c, w, hb_heads, block);
+  else join_many(c, w, hb_heads, block, joins);
 }
 
 int check_decode(const akl_decode_t* c, akl_decode_layout_t* L) {
@@ -960,7 +1037,8 @@ int akl_paged_decode(const akl_decode_t* c, void* stream) {
     rc = hb == 4 ? launch_decode<AKL_KV_FP16, 4>(*c, w, ctas, s)
                  : (hb == 2 ? launch_decode<AKL_KV_FP16, 2>(*c, w, ctas, s) : launch_decode<AKL_KV_FP16, 1>(*c, w, ctas, s));
   if (rc != AKL_OK) return rc;
-  // the wide join while its CTAs fit the GPU in about two waves; past that a request has few parts
+  // the wide join while its CTAs fit the GPU in about two waves; past that most requests have few parts, and join_many
+  // looks which have not
   const int64_t pairs = static_cast<int64_t>(c->batch) * c->q_heads;
   const bool wide = pairs * 4 <= 8 * sms;
   const int64_t joins = wide ? pairs * 4 : (pairs + 7) / 8;

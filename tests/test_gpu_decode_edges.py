@@ -218,3 +218,21 @@ def test_weights_of_rows_whose_products_are_exact(pkg, cuda, dtype):
     # what longer products lose; three roundings of the factor and the exponent's argument besides
     size = float(x.amax()) * R.LOG2E
     assert float(((got.double() - want).abs() / want.clamp(min=1e-3)).max()) <= math.log(2) * size * (2.0 ** -22 + 5 * 2.0 ** -24) + 1e-5
+
+
+@pytest.mark.parametrize("lens,heads,dtype", [
+    ([30000] + [3] * 12, (24, 4), BF16), ([2] * 30 + [9000, 1, 7000, 0] + [5] * 20 + [20000], (24, 4), FP16),
+    ([4000] * 12 + [1] * 300, (6, 1), BF16), ([1] * 40 + [33000], (64, 8), BF16), ([12000] + [0] * 200 + [300] * 3, (8, 2), FP16),
+], ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_long_requests_among_many_short_ones(pkg, cuda, lens, heads, dtype):
+    """Parts of one request in nearly every CTA, and more (request, head) pairs than the wide join takes."""
+    c = R.case(lens, *heads, dtype=dtype, seed=len(lens))
+    weights = torch.zeros(c["page_table"].shape, device=cuda)
+    ws = pkg.plan_decode_workspace(cuda, max_requests=len(lens), q_heads=heads[0], kv_heads=heads[1],
+                                   max_weight_tokens=sum(lens) + 64 * len(lens))
+    got = [pkg.paged_decode(**c, workspace=ws, return_lse=True, weights=weights, weight_decay=0.0, check_status=True) for _ in range(2)]
+    ref = R.decode(c["q"], c["k_pool"], c["v_pool"], c["page_table"], c["kv_lens"], c["rows"], weights=torch.zeros_like(weights))
+    R.within(got[0][0], ref["out"], ref["out_tol"])
+    R.within(got[0][1], ref["lse"], ref["lse_tol"])
+    R.within(weights, ref["weights"], ref["weights_tol"])
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
