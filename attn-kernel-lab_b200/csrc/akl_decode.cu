@@ -19,9 +19,10 @@
 //     forms the scores, half the products each, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
 //     heads of the kv head on N -- with the heads on M half to three quarters of the tensor work would
 //     be padding.  Out^T = V^T P^T takes P^T in the operand layout that an 8x8 transpose of the score
-//     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: a tile needs 8192
-//     multiply-adds per position and kv head against the ~43 cycles that its bytes take per SM (the tensor
-//     pipe is 9 to 13 % busy); tcgen05's 128 rows would be 6 to 25 % filled and its TMEM round trip longer.
+//     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: 6144
+//     multiply-adds per position and kv head (2048 for eight heads' scores, twice that for the two parts of P)
+//     against the ~43 cycles that its bytes take per SM (the tensor pipe is 9 to 13 % busy); tcgen05's 128 rows would
+//     be 6 to 25 % filled and its TMEM round trip longer.
 //
 // Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 364 to 368 us, 92 to 93 % of the
 // copy bandwidth; one request of 139264 positions, 571 MB, 104 to 109 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,

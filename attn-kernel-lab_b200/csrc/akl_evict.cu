@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const akl_evict_t c,
         const uint32_t total = __reduce_add_sync(0xffffffffu, sm.counts[warp][lane]);
         if (lane == 0) sm.totals[round & 1][warp] = total;
       }
-      cluster.sync();                                   // every weight of the round is in a register
+      cluster.sync();                                   // the totals are there; the round's keys are in shared memory
     }
     for (int g = 0; g < groups; ++g) {
         const int at = start_of(g);

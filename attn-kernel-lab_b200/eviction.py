@@ -279,6 +279,8 @@ def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: in
     equal weights the lowest positions stay).  What stays moves to the front of its row in position
     order, slots and weights alike; the weights behind it, up to the old length, become 0; table entries
     behind it are left as they were.  A shorter request keeps its row.  Requests must name distinct rows.
+    A length is cut to the table's width, and what comes back for it is at most that; for a length below 0 or
+    a row outside the table it is 0.
 
     By default `page_table`, `weights` and `kv_lens` are changed in place; `page_table_out`,
     `weights_out` and `kv_lens_out` of the same shapes take the result instead (other rows, and what lies
