@@ -24,9 +24,9 @@
 //     against the ~43 cycles that its bytes take per SM (the tensor pipe is 9 to 13 % busy); tcgen05's 128 rows would
 //     be 6 to 25 % filled and its TMEM round trip longer.
 //
-// Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 364 to 368 us, 92 to 93 % of the
-// copy bandwidth; one request of 139264 positions, 571 MB, 104 to 109 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
-// 8.7 us.  The short ones are bound by three dependent trips to memory (lengths, page table, rows) and the join,
+// Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 359 us, 95 % of the
+// copy bandwidth; one request of 139264 positions, 571 MB, 103 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
+// 9.0 us.  The short ones are bound by three dependent trips to memory (lengths, page table, rows) and the join,
 // the long ones by HBM and by the SMs that get their equal share up to 8 % later than the median.
 //
 // Rounding: scores, m, l and both sums are 32-bit.  P enters the second product as two 16-bit parts,

@@ -14,10 +14,11 @@
 // rounds, their weights read again for each digit (from L2).  Rows may be shortened in place: positions only
 // move forward, and what a group of 8192 positions a CTA overwrites has been read by all when its barrier opens.
 //
-// Few bytes and two or three dependent passes.  One request of 139264 positions (16 CTAs) takes 21 us, of which
+// Few bytes and two or three dependent passes.  One request of 139264 positions (16 CTAs) takes 21 to 24 us, of which
 // memory would be 0.5: two or three passes with two cluster barriers each, about a microsecond apiece, and the trips to
-// L2.  256 requests of up to 32768 take 38 to 39 us, memory 10: about 6 us a request whatever its length and 0.6 ns a
-// position, at 60 % of the issue slots.
+// L2.  256 requests of up to 32768 take 37 to 38 us, memory 10: about 6 us a request whatever its length and 0.6 ns a
+// position, at 60 % of the issue slots.  In place, which needs a barrier a group and leaves the requests in the order
+// given, 26 and 41 us.
 #include <cooperative_groups.h>
 
 #include <atomic>
