@@ -114,7 +114,7 @@ def extend_weights(q, k_pool, idx, prefix, lse, weights, *, weight_decay: float 
         sum over t, h with i <= prefix + t of 2^(sm_scale log2e <q[t, h], k_i> - lse[t, h]).
 
     A row whose `lse` is infinite adds nothing, whatever its `q` holds (it saw no key); a key that is not finite
-    makes its own position's weight NaN as soon as a row sees it, and no other's; a slot outside the pool gets no weight.
+    can make its own position's weight NaN, and no other's; a slot outside the pool gets no weight.
     `weights` shares no memory with an input.
     To judge by a window of w rows pass `q[-w:]`, `lse[-w:]` and `prefix + q_len - w`.  The sum has a
     fixed order: equal inputs give equal bits.
@@ -285,7 +285,8 @@ def evict_lightest(page_table, weights, kv_lens, *, keep: int, protect_first: in
     By default `page_table`, `weights` and `kv_lens` are changed in place; `page_table_out`,
     `weights_out` and `kv_lens_out` of the same shapes take the result instead (other rows, and what lies
     behind a request's old length, stay as they are).  But for that, no output shares memory with an input or
-    another output; a table and its weights may lie side by side in one buffer.  `freed` [batch, >= width - keep] receives the
+    another output; a table and its weights may lie side by side in one buffer.
+    `freed` [batch, >= width - keep] receives the
     slots that go, in position order, and `freed_lens` [batch] int32 their number; both are allocated
     when not given.  Enqueues on the current stream and does not synchronise.
 

@@ -24,6 +24,13 @@ def test_pool_lse_belongs_to_a_returned_lse(pkg):
             call(pool_lse=1, return_lse=True)
         with pytest.raises(RuntimeError, match="no CPU path"):
             call(pool_lse=True, return_lse=True)
+    r = _request()
+    paged = (r["q"], r["k_pool"][:, None], r["v_pool"][:, None], r["idx"])
+    with pytest.raises(pkg.CapabilityError) as e:
+        pkg.fp8_paged_prefill(*paged, pool_lse=True)
+    assert e.value.field == "pool_lse"
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        pkg.fp8_paged_prefill(*paged, pool_lse=True, return_lse=True)
 
 
 def test_flag_matches_the_header_and_travels(pkg):
