@@ -19,23 +19,24 @@
 //     forms the scores, half the products each, S^T = K Q^T as m16n8k16 with the positions on M and the (up to eight) q
 //     heads of the kv head on N -- with the heads on M half to three quarters of the tensor work would
 //     be padding.  Out^T = V^T P^T takes P^T in the operand layout that an 8x8 transpose of the score
-//     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: 6144
-//     multiply-adds per position and kv head (2048 for eight heads' scores, twice that for the two parts of P)
-//     against the ~43 cycles that its bytes take per SM (the tensor pipe is 9 to 13 % busy); tcgen05's 128 rows would
-//     be 6 to 25 % filled and its TMEM round trip longer.
+//     fragment gives, so P never touches shared memory.  mma.sync, not tcgen05: 8192
+//     multiply-adds per position and kv head (2048 for eight heads' scores, three times that for the parts of P; two
+//     times for an FP16 pool) against the ~43 cycles that its bytes take per SM (the tensor pipe is 12 to 17 % busy);
+//     tcgen05's 128 rows would be 6 to 25 % filled and its TMEM round trip longer.
 //
 // Measured (a call in a CUDA graph): 64 ragged requests, 2.2 GB of K and V, 359 us, 95 % of the
-// copy bandwidth; one request of 139264 positions, 571 MB, 103 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
+// copy bandwidth; one request of 139264 positions, 571 MB, 103 to 106 us; 8 requests, 137 MB, 36 us; one of 1000, 4 MB,
 // 9.0 us.  The short ones are bound by three dependent trips to memory (lengths, page table, rows) and the join,
 // the long ones by HBM and by the SMs that get their equal share up to 8 % later than the median.
 //
-// Rounding: scores, m, l and both sums are 32-bit.  P enters the second product as two 16-bit parts,
-// p = hi + lo (2^-16 relative): with one part alone the error of the outputs was 1.77e-3 instead of 1.66e-3, which
-// is the BF16 rounding of the result, and the extra products took no time that shows.  The tensor pipe cuts its
+// Rounding: scores, m, l and both sums are 32-bit, and so is P: it enters the second product as a sum of three BF16
+// numbers, or of two FP16 ones, 24 and 22 bits.  (With one the error of the outputs was 1.77e-3 instead of 1.66e-3, which
+// is the BF16 rounding of the result; with two of BF16, 17 bits, one output in 1000 was not the correctly rounded one,
+// with three one in 4000.  The third takes 1 % of the time.)  The tensor pipe cuts its
 // 32-bit sums off where it should round, always towards zero, and over a thousand tiles that adds up; so it sums
 // within a tile only, from zero, and the tiles are added up by FMAs that round.  (Distance of the outputs from the
-// correctly rounded ones in the long cases: 1.3e-4 to 1.5e-4 with one running sum, 0.2e-4 to 0.7e-4 so, for 0 to 0.6 %
-// of the time.)  For an FP16 pool P is
+// correctly rounded ones in the long cases: 1.3e-4 to 1.5e-4 with one running sum and two parts, below 0.5e-4 now, for 0 to
+// 0.6 % of the time.)  For an FP16 pool P is
 // scaled by 2^14, so that small probabilities stay normal numbers, and Q (BF16) is brought to FP16 by the power
 // of two of its row's largest element: exact down to 2^-17 of that element, 2^-25 of it below.
 #include <algorithm>
@@ -258,24 +259,25 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two floats to the pool's type, and what that rounding left of them.
-template <int KV>
-__device__ __forceinline__ uint32_t split2(float a, float b, uint32_t& rest) {
-  uint32_t hi;
-  if (KV == AKL_KV_BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const float2 f = __bfloat1622float2(h);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    rest = *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    rest = *reinterpret_cast<const uint32_t*>(&r);
+// Two floats as sums of numbers of the pool's type, the largest first.
+template <int KV, int kParts>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&out)[kParts][2], int at) {
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    if (KV == AKL_KV_BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+      const float2 f = __bfloat1622float2(h);
+      out[i][at] = *reinterpret_cast<const uint32_t*>(&h);
+      a -= f.x;
+      b -= f.y;
+    } else {
+      const __half2 h = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(h);
+      out[i][at] = *reinterpret_cast<const uint32_t*>(&h);
+      a -= f.x;
+      b -= f.y;
+    }
   }
-  return hi;
 }
 
 // Queries of one kv head as the B operand, channels 128 half ..: thread (g, q) = (lane / 4, lane % 4) holds head g,
@@ -432,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
   const int g = lane >> 2, quad = lane & 3, group = c.q_heads / c.kv_heads;
   const uint32_t bars = smem + T::kOffBar;
   constexpr float kShift = KV == AKL_KV_FP16 ? 14.f : 0.f;   // P carries 2^kShift
+  constexpr int kParts = KV == AKL_KV_BF16 ? 3 : 2;          // numbers of the pool's type that make up one of P
   const uint32_t k_lane = (tg * 16 + (lane & 15)) * T::kPitch + unit * 512 + half * 256 + (lane >> 4) * 16;
   const uint32_t v_lane = T::kPlane + (tg * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * T::kPitch + unit * 512 + half * 256 +
                           ((lane >> 3) & 1) * 16;
@@ -523,19 +526,21 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const akl_decode_t 
         for (int i = 0; i < 4; ++i) p[i] = ex2(x[i] - safe[i & 1] + kShift);
         l[0] = fmaf(l[0], alpha[0], p[0] + p[2]);
         l[1] = fmaf(l[1], alpha[1], p[1] + p[3]);
-        uint32_t lo0, lo1;
-        uint32_t hi0 = split2<KV>(p[0], p[1], lo0), hi1 = split2<KV>(p[2], p[3], lo1);
-        hi0 = transpose8x8(hi0);
-        hi1 = transpose8x8(hi1);
-        lo0 = transpose8x8(lo0);
-        lo1 = transpose8x8(lo1);
+        uint32_t pt[kParts][2];
+        split2<KV>(p[0], p[1], pt, 0);
+        split2<KV>(p[2], p[3], pt, 1);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          pt[i][0] = transpose8x8(pt[i][0]);
+          pt[i][1] = transpose8x8(pt[i][1]);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint32_t a[4];
           ldsm4_trans(stage + v_lane + i * 32, a);
           float t[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16<KV>(t, a, lo0, lo1);
-          mma16<KV>(t, a, hi0, hi1);
+#pragma unroll
+          for (int k = kParts - 1; k >= 0; --k) mma16<KV>(t, a, pt[k][0], pt[k][1]);
           o[i][0] = fmaf(o[i][0], alpha[0], t[0]);
           o[i][1] = fmaf(o[i][1], alpha[1], t[1]);
           o[i][2] = fmaf(o[i][2], alpha[0], t[2]);

@@ -236,3 +236,32 @@ def test_long_requests_among_many_short_ones(pkg, cuda, lens, heads, dtype):
     R.within(got[0][1], ref["lse"], ref["lse_tol"])
     R.within(weights, ref["weights"], ref["weights_tol"])
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_probabilities_keep_their_32_bits_in_the_second_product(pkg, cuda, dtype):
+    """Three positions with the values 0, 1 and -1, so an output is (p1 - p2) / l, a difference of nearly equal numbers.
+
+    p1 and p2 lie about 0.53 to 0.73 and 2^-13 apart.  Their exponentials are off by 2^-22 of themselves, their scores
+    (of one product and a small one, so next to exact) by two roundings of 2^-25; l is at least 2.  So the output, below
+    2^-13 and rounded to 2^-9 of itself, is off by 2 * 0.73 / 2 * (2^-22 + 2^-24) and 2^-22 at most: by 2^-21.  In two numbers of
+    eight bits a probability would be off by up to 2^-18."""
+    g = torch.Generator().manual_seed(9)
+    batch, heads, kv = 200, 24, 4
+    q = torch.zeros((batch, heads, 256))
+    q[:, :, 0] = 1 + torch.randint(0, 128, (batch, heads), generator=g) / 128
+    q[:, :, 1] = 2.0 ** -12 * torch.randint(-128, 129, (batch, heads), generator=g) / 128
+    k = torch.zeros((batch, 3, kv, 256))
+    k[:, 0, :, 0], k[:, 1:, :, 0] = 8.0, 3.0
+    k[:, 1, :, 1] = torch.randint(1, 9, (batch, kv), generator=g).float()
+    k[:, 2, :, 1] = -torch.randint(1, 9, (batch, kv), generator=g).float()
+    v = torch.tensor([0.0, 1.0, -1.0])[None, :, None, None].expand(batch, 3, kv, 256)
+    pool = [t.reshape(3 * batch, kv, 256).to(dtype).to(cuda) for t in (k, v)]
+    table = torch.arange(3 * batch, device=cuda).view(batch, 3)
+    out = pkg.paged_decode(q.to(BF16).to(cuda), *pool, table, torch.full((batch,), 3, device=cuda))
+    x = torch.einsum("bjgd,bnjd->bjgn", q.double().view(batch, kv, heads // kv, 256), k.double()).reshape(batch, heads, 3) / 16
+    p = torch.softmax(x, -1)
+    want = (p[:, :, 1] - p[:, :, 2]).to(cuda)
+    assert float(want.abs().max()) < 2.0 ** -13 and float(p[:, :, 0].max()) < 0.5
+    worst = float((out.double() - want[:, :, None]).abs().max())
+    assert worst <= 2.0 ** -21, f"2^{math.log2(worst):.2f}"
